@@ -41,7 +41,8 @@ enum {
   VLA_E_CUDA = -3,         /* a CUDA runtime / driver call failed */
   VLA_E_UNSUPPORTED = -4,  /* valid request this build does not implement */
   VLA_E_DEVICE_TIMEOUT = -5, /* a kernel's bounded wait expired (see vla_sync_check) */
-  VLA_E_WORKSPACE = -6     /* workspace too small */
+  VLA_E_WORKSPACE = -6,    /* workspace too small */
+  VLA_E_DEVICE_RANGE = -7  /* a kernel skipped a cache position or page out of range (see vla_sync_check) */
 };
 
 /* Activation / epilogue kinds of vla_gemm_bf16. */
@@ -88,7 +89,7 @@ typedef struct vla_epilogue {
 const char* vla_last_error(void);
 int vla_version(void);
 /* Synchronises the current device, then reads and clears the device error
- * word.  Returns VLA_OK, VLA_E_DEVICE_TIMEOUT or VLA_E_CUDA. */
+ * word.  Returns VLA_OK, VLA_E_DEVICE_TIMEOUT, VLA_E_DEVICE_RANGE or VLA_E_CUDA. */
 int vla_sync_check(void);
 /* Device error word without clearing (0 = none). */
 int vla_peek_device_error(unsigned int* code);
@@ -287,6 +288,90 @@ enum {
   VLA_ATTN_TCGEN05_PIPE = 4
 };
 int vla_attention_bf16(const vla_attention_args* a, vla_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Quantised key/value cache                                               */
+/* ---------------------------------------------------------------------- */
+
+/* Keys and values of sequences that grow, held in 4 or 8 bits: a pool of pages
+ * of VLA_KV_PAGE tokens, page numbers per sequence in a table, so sequences grow
+ * without moving.  A page holds one block of vla_kv_block_bytes(bits) bytes per
+ * kv head (pool: [pages][kv_heads][block bytes], 16-byte aligned).  Block: key
+ * codes | value codes | scales (2048 + 2048 + 512 bytes in 4 bits, 4096 + 4096 +
+ * 512 in 8); a token's 64 key (and value) elements are two groups of 32 with a
+ * bf16 scale each.
+ *   4 bits: scale d = the element of largest magnitude over -8 (the positive
+ *           sign when both signs reach it or it is 0), its magnitude rounded up
+ *           to 5 significant bits; code = rint(x / d) (ties to even) in [-8, 7],
+ *           stored plus 8;
+ *   8 bits: d = the smallest power of two with 127 d >= the largest magnitude,
+ *           code = rint(x / d), two's complement.
+ * |d| >= 2^-100; a group with a NaN, an infinity or a magnitude of 2^127 or more
+ * has d = NaN and reads back as NaN.  code * d is a bf16 number exactly.
+ * The order of a block's codes and scales (tiles of 16 tokens in the order of
+ * the tensor-core operands) is written out in csrc/kvcache.cuh.
+ * Token j of sequence b is in page table[b * table_ld + j / 64], at j % 64.  A
+ * table entry outside [0, pages), or a position outside the table, is skipped
+ * by the kernels (its keys are not seen, its rows neither written nor read) and
+ * reported by vla_sync_check as VLA_E_DEVICE_RANGE.
+ * No counterpart in the reference, whose blocks recompute keys and values. */
+#define VLA_KV_PAGE 64
+typedef struct vla_kv_cache {
+  void* pool;
+  const int32_t* table;   /* device [batch][table_ld] */
+  int64_t table_ld;
+  int32_t pages;          /* pages in the pool */
+  int32_t max_pages;      /* table columns: a sequence holds at most 64 * max_pages tokens */
+  int32_t batch, kv_heads;
+  int32_t head_dim;       /* 64 */
+  int32_t bits;           /* 4 or 8 */
+} vla_kv_cache;
+size_t vla_kv_block_bytes(int32_t bits);
+
+/* Quantises K and V rows into the cache: row i < min(n, count[b]) of sequence b
+ * (kv_heads * 64 bf16 at k + b * k_batch + i * k_row; the same for v) becomes
+ * token start[b] + i.  start: device int32 [batch]; count: device int32 [batch]
+ * or NULL (n).  Lengths are the caller's: nothing else changes, so the layers
+ * of a model write at one and the same start. */
+int vla_kv_append_bf16(const vla_kv_cache* c, const void* k, int64_t k_row, int64_t k_batch, const void* v,
+                       int64_t v_row, int64_t v_batch, int32_t n, const int32_t* start, const int32_t* count,
+                       vla_stream_t stream);
+
+/* The bf16 keys and values that the cache stands for: token start[b] + i (start
+ * NULL: 0) to row i < n of sequence b; rows i >= count[b] (NULL: n) are written
+ * as zeros. */
+int vla_kv_read_bf16(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, void* v, int64_t v_row,
+                     int64_t v_batch, int32_t n, const int32_t* start, const int32_t* count, vla_stream_t stream);
+
+/* Attention of Lq query tokens per sequence over its cache, O = softmax(scale
+ * Q K^T) V per head; query head h reads kv head h * kv_heads / Hq.  Sequence b
+ * holds lens[b] tokens, of which its query tokens are the newest: token i of
+ * q_len[b] (NULL: Lq) valid ones has the position lens[b] - q_len[b] + i if
+ * causal, else every one has lens[b] - 1.  A query at position p sees key j <= p
+ * when window == 0 or j > p - window or j < sinks.  Rows that see no key, and
+ * rows i >= q_len[b], are written as zeros.  Keys that are not seen have no
+ * effect, whatever their memory holds.
+ * max_len (0: the table's capacity) is an upper bound of lens that the split of
+ * the work is made for; longer sequences stay right.  The workspace
+ * (vla_kv_attention_workspace bytes, 16-byte aligned; 0: none) holds the parts'
+ * sums and belongs to one call at a time. */
+typedef struct vla_kv_attention_args {
+  const void* q;
+  void* o;
+  int64_t q_row, q_batch, o_row, o_batch;
+  const int32_t* lens;   /* device int32 [batch] */
+  const int32_t* q_len;  /* device int32 [batch] or NULL */
+  int32_t Lq, Hq;
+  int32_t causal;
+  int32_t window, sinks;
+  int32_t max_len;
+  float scale;
+  int32_t reserved;
+  void* workspace;
+  size_t workspace_bytes;
+} vla_kv_attention_args;
+size_t vla_kv_attention_workspace(const vla_kv_cache* c, const vla_kv_attention_args* a);
+int vla_kv_attention_bf16(const vla_kv_cache* c, const vla_kv_attention_args* a, vla_stream_t stream);
 
 /* Pixel shuffle: in [B, grid*grid, C] -> out [B, (grid/s)^2, s*s*C] with
  * out[b, (h/s)*(grid/s) + w/s, (h%s)*s*C + (w%s)*C + c] = in[b, h*grid + w, c]

@@ -1,0 +1,206 @@
+// Host side of the quantised key/value cache: argument checks, the choice of
+// row tile and key splits, launches.
+#pragma once
+#include <cmath>
+
+#include "host_common.cuh"
+#include "kv_attention.cuh"
+#include "kvcache.cuh"
+
+namespace vla {
+namespace kv {
+
+static size_t block_bytes(int bits) {
+  return bits == 4 ? (size_t)Block<4>::kBytes : bits == 8 ? (size_t)Block<8>::kBytes : 0;
+}
+
+static int check_cache(const vla_kv_cache* c, const char* what) {
+  VLA_CHECK_ARG(c != nullptr, "%s: null cache", what);
+  VLA_CHECK_ARG(c->bits == 4 || c->bits == 8, "%s: a cache holds 4 or 8 bits, not %d", what, c->bits);
+  VLA_CHECK_ARG(c->head_dim == HD, "%s: head_dim must be 64", what);
+  VLA_CHECK_ARG(c->batch >= 0 && c->kv_heads > 0 && c->pages >= 0 && c->max_pages >= 0, "%s: bad cache shape", what);
+  VLA_CHECK_ARG((long long)c->max_pages * kPage < (1ll << 31), "%s: %d pages per sequence are 2^31 tokens or more",
+                what, c->max_pages);
+  VLA_CHECK_ARG(c->table_ld >= c->max_pages, "%s: table stride %lld below its %d columns", what,
+                (long long)c->table_ld, c->max_pages);
+  VLA_CHECK_ARG(c->batch == 0 || (c->pool != nullptr && c->table != nullptr), "%s: null pool or table", what);
+  VLA_CHECK_ALIGN(aligned16(c->pool), "%s: the pool must be 16-byte aligned", what);
+  return VLA_OK;
+}
+
+static Cache device_cache(const vla_kv_cache* c) {
+  return Cache{(uint8_t*)c->pool, c->table, (long long)c->table_ld, c->pages, c->max_pages, c->batch, c->kv_heads};
+}
+
+// Row tensors [batch][n] of kv_heads * 64 (or heads * 64) elements.
+static int check_rows(const void* x, int64_t row, int64_t batch, int64_t width, const char* what, const char* name) {
+  VLA_CHECK_ARG(x != nullptr, "%s: null %s", what, name);
+  VLA_CHECK_ARG(row >= width && batch >= 0, "%s: %s rows of stride %lld hold %lld elements", what, name,
+                (long long)row, (long long)width);
+  VLA_CHECK_ALIGN(aligned16(x) && row % 8 == 0 && batch % 8 == 0, "%s: 16-byte alignment of %s and its strides", what,
+                  name);
+  return VLA_OK;
+}
+
+#define VLA_TRY(expr)                \
+  do {                               \
+    const int _rc = (expr);          \
+    if (_rc != VLA_OK) return _rc;   \
+  } while (0)
+
+static int append(const vla_kv_cache* c, const void* k, int64_t k_row, int64_t k_batch, const void* v, int64_t v_row,
+                  int64_t v_batch, int32_t n, const int32_t* start, const int32_t* count, cudaStream_t st) {
+  VLA_TRY(check_cache(c, "kv_append"));
+  VLA_CHECK_ARG(n >= 0, "kv_append: n must not be negative");
+  if (c->batch == 0 || n == 0) return VLA_OK;
+  VLA_CHECK_ARG(start != nullptr, "kv_append: null start");
+  const int64_t width = (int64_t)c->kv_heads * HD;
+  VLA_TRY(check_rows(k, k_row, k_batch, width, "kv_append", "k"));
+  VLA_TRY(check_rows(v, v_row, v_batch, width, "kv_append", "v"));
+  AppendParams p{device_cache(c), (const bf16*)k, (const bf16*)v, (long long)k_row, (long long)v_row,
+                 (long long)k_batch, (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4)};
+  const long long items = (long long)c->batch * p.quads * c->kv_heads;
+  VLA_CHECK_ARG((long long)p.quads * c->kv_heads < (1ll << 31) && (items + 7) / 8 < (1ll << 31),
+                "kv_append: too many rows");
+  prof_begin(st);
+  launch_k(c->bits == 4 ? append_kernel<4> : append_kernel<8>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, p,
+           items);
+  prof_end(st, VLA_KIND_LAYOUT, 0.0,
+           (double)c->batch * n * c->kv_heads * (4.0 * HD + (double)block_bytes(c->bits) / kPage));
+  return launch_status("kv_append");
+}
+
+static int read(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, void* v, int64_t v_row,
+                int64_t v_batch, int32_t n, const int32_t* start, const int32_t* count, cudaStream_t st) {
+  VLA_TRY(check_cache(c, "kv_read"));
+  VLA_CHECK_ARG(n >= 0, "kv_read: n must not be negative");
+  if (c->batch == 0 || n == 0) return VLA_OK;
+  const int64_t width = (int64_t)c->kv_heads * HD;
+  VLA_TRY(check_rows(k, k_row, k_batch, width, "kv_read", "k"));
+  VLA_TRY(check_rows(v, v_row, v_batch, width, "kv_read", "v"));
+  ReadParams p{device_cache(c), (bf16*)k, (bf16*)v, (long long)k_row, (long long)v_row, (long long)k_batch,
+               (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4)};
+  const long long items = (long long)c->batch * p.quads * c->kv_heads;
+  VLA_CHECK_ARG((long long)p.quads * c->kv_heads < (1ll << 31) && (items + 7) / 8 < (1ll << 31),
+                "kv_read: too many rows");
+  prof_begin(st);
+  launch_k(c->bits == 4 ? read_kernel<4> : read_kernel<8>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, p,
+           items);
+  prof_end(st, VLA_KIND_LAYOUT, 0.0,
+           (double)c->batch * n * c->kv_heads * (4.0 * HD + (double)block_bytes(c->bits) / kPage));
+  return launch_status("kv_read");
+}
+
+// Row tile and key splits of a call; both depend on its sizes alone.
+struct Plan {
+  int nt, row_blocks, parts, per;
+  size_t workspace;
+};
+
+static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a, Plan* out) {
+  const long long rows = (long long)a->Lq * (a->Hq / c->kv_heads);
+  VLA_CHECK_ARG(rows < (1ll << 30), "kv_attention: too many query rows");
+  out->nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  out->row_blocks = (int)((rows + 8 * out->nt - 1) / (8 * out->nt));
+  const long long room = (long long)c->max_pages * kPage;
+  long long keys = a->max_len > 0 && a->max_len < room ? a->max_len : room;
+  if (a->window > 0) {
+    // the window of a block's rows and the first tokens, at 32-key granularity
+    const long long seen = (long long)a->window + a->sinks + (8 * out->nt - 1) / (a->Hq / c->kv_heads) + 3 * kUnit;
+    if (seen < keys) keys = seen;
+  }
+  const long long units = (keys + kUnit - 1) / kUnit;
+  const long long base = (long long)c->batch * c->kv_heads * out->row_blocks;
+  const long long want = (12ll * device_info().num_sms + base - 1) / base;
+  const long long most = (units + 15) / 16;
+  long long parts = want < most ? want : most;
+  if (parts < 1) parts = 1;
+  out->per = (int)((units + parts - 1) / parts);
+  if (out->per < 1) out->per = 1;
+  out->parts = (int)parts;
+  VLA_CHECK_ARG(base * parts < (1ll << 31), "kv_attention: too many work items");
+  out->workspace = parts > 1 ? (size_t)base * parts * 8 * out->nt * (HD + 2) * sizeof(float) : 0;
+  return VLA_OK;
+}
+
+static int check_attention(const vla_kv_cache* c, const vla_kv_attention_args* a) {
+  VLA_TRY(check_cache(c, "kv_attention"));
+  VLA_CHECK_ARG(a != nullptr, "kv_attention: null args");
+  VLA_CHECK_ARG(a->Lq >= 0 && a->Hq > 0 && a->Hq % c->kv_heads == 0, "kv_attention: %d query heads over %d kv heads",
+                a->Hq, c->kv_heads);
+  VLA_CHECK_ARG(a->window >= 0 && a->sinks >= 0 && a->max_len >= 0, "kv_attention: negative window, sinks or max_len");
+  VLA_CHECK_ARG(std::isfinite(a->scale) && a->scale > 0.f, "kv_attention: scale must be positive and finite");
+  return VLA_OK;
+}
+
+template <int BITS, int NT>
+static void launch_attend(const AttnParams& p, const Plan& pl, cudaStream_t st) {
+  const long long base = (long long)p.c.batch * p.c.kv_heads * pl.row_blocks;
+  launch_k(attend_kernel<BITS, NT>, dim3((unsigned)(base * pl.parts)), dim3(kWarps * 32), 0, st, p);
+  if (pl.parts > 1) launch_k(join_kernel<NT>, dim3((unsigned)base), dim3(256), 0, st, p);
+}
+
+static size_t attention_workspace(const vla_kv_cache* c, const vla_kv_attention_args* a) {
+  Plan pl;
+  if (check_attention(c, a) != VLA_OK || c->batch == 0 || a->Lq == 0) return 0;
+  return plan_attention(c, a, &pl) == VLA_OK ? pl.workspace : 0;
+}
+
+static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cudaStream_t st) {
+  VLA_TRY(check_attention(c, a));
+  if (c->batch == 0 || a->Lq == 0) return VLA_OK;
+  VLA_CHECK_ARG(a->lens != nullptr, "kv_attention: null lens");
+  VLA_TRY(check_rows(a->q, a->q_row, a->q_batch, (int64_t)a->Hq * HD, "kv_attention", "q"));
+  VLA_TRY(check_rows(a->o, a->o_row, a->o_batch, (int64_t)a->Hq * HD, "kv_attention", "o"));
+  Plan pl;
+  VLA_TRY(plan_attention(c, a, &pl));
+  if (pl.workspace > 0) {
+    if (a->workspace == nullptr || a->workspace_bytes < pl.workspace)
+      return set_error(VLA_E_WORKSPACE, "kv_attention: needs %zu bytes of workspace, got %zu", pl.workspace,
+                       a->workspace == nullptr ? (size_t)0 : a->workspace_bytes);
+    VLA_CHECK_ALIGN(aligned16(a->workspace), "kv_attention: workspace alignment");
+  }
+  AttnParams p{};
+  p.c = device_cache(c);
+  p.q = (const bf16*)a->q;
+  p.o = (bf16*)a->o;
+  p.q_row = a->q_row;
+  p.q_batch = a->q_batch;
+  p.o_row = a->o_row;
+  p.o_batch = a->o_batch;
+  p.lens = a->lens;
+  p.q_len = a->q_len;
+  p.Lq = a->Lq;
+  p.Hq = a->Hq;
+  p.G = a->Hq / c->kv_heads;
+  p.causal = a->causal != 0;
+  // a window as long as the cache hides nothing, and first tokens mean nothing without one
+  const long long room = (long long)c->max_pages * kPage;
+  p.window = a->window > 0 && a->window < room ? a->window : 0;
+  p.sinks = a->sinks < room ? a->sinks : (int)room;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.row_blocks = pl.row_blocks;
+  p.parts = pl.parts;
+  p.per = pl.per;
+  p.part_o = (float*)a->workspace;
+  if (pl.parts > 1)
+    p.part_ml = p.part_o + (size_t)c->batch * c->kv_heads * pl.row_blocks * pl.parts * 8 * pl.nt * HD;
+  prof_begin(st);
+  if (c->bits == 4) {
+    if (pl.nt == 1) launch_attend<4, 1>(p, pl, st);
+    else if (pl.nt == 2) launch_attend<4, 2>(p, pl, st);
+    else launch_attend<4, 4>(p, pl, st);
+  } else {
+    if (pl.nt == 1) launch_attend<8, 1>(p, pl, st);
+    else if (pl.nt == 2) launch_attend<8, 2>(p, pl, st);
+    else launch_attend<8, 4>(p, pl, st);
+  }
+  // the lengths are on the device: the profile counts whole caches (or windows)
+  const double keys = (double)pl.per * pl.parts * kUnit;
+  prof_end(st, VLA_KIND_ATTENTION, 4.0 * c->batch * a->Hq * (double)a->Lq * keys * HD,
+           c->batch * (keys * c->kv_heads * block_bytes(c->bits) / kPage + 4.0 * a->Lq * a->Hq * HD));
+  return launch_status("kv_attention");
+}
+
+}  // namespace kv
+}  // namespace vla

@@ -1,0 +1,361 @@
+// Quantised key/value cache, head_dim 64: the block layout, the kernel that
+// quantises rows as it writes them and the one that reads them back.
+//
+// A cache is a pool of pages of 64 tokens; a page holds one block per kv head.
+// Block: key codes | value codes | scales (4 bits: 2048 + 2048 + 512 bytes,
+// 8 bits: 4096 + 4096 + 512 bytes), tokens in tiles of 16.
+//
+// Quantisation of a group of 32 elements (two groups per row of 64), a = max |x|:
+//   4 bits: d = a / 8 with its magnitude rounded UP to 5 significant bits, so
+//           that |x / d| <= 8; d is negative when the largest magnitude is a
+//           positive element only, so that it takes code -8 (the code range
+//           [-8, 7] has one more negative code);
+//           code = min(rint(x / d), 7), stored plus 8.
+//   8 bits: d = the smallest power of two with 127 d >= a; code = rint(x / d).
+// d >= 2^-100; d = NaN when a is not below 2^127 (NaN and infinities included).
+// A 4-bit code has at most 3 significant bits and a 4-bit d five, an 8-bit
+// code at most 7 and an 8-bit d one, so code * d is a bf16 number EXACTLY: the
+// cache stands for bf16 keys and values, and every reader (this file's, and the
+// attention kernels' products with the scales applied before or after) sees the
+// same numbers without another rounding.
+//
+// Order inside a tile.  The attention kernel feeds keys and values to
+// mma.m16n8k16 as the 16-row operand, straight from global memory to registers:
+// lane (g = lane / 4, t = lane % 4) needs for its key rows g and g + 8 the same
+// 16 dims, and for its value columns 2t, 2t+1, 2t+8, 2t+9 (tokens) the same 8
+// dims.  Rows are taken as tokens 4(g/2) + g%2 and that + 2, columns as tokens
+// 4t .. 4t+3, which makes both a 16-byte load per lane, contiguous over the warp:
+//   keys   4 bits: 16 bytes at (2q + b) * 64 + t * 16 = [token 4q+b: word of
+//          dims 8t.. of group 0, of group 1; token 4q+b+2: the same]
+//   values 4 bits: 16 bytes at q * 128 + g * 16 = [word of token 4q + r: dims
+//          4g..4g+3 of group 0, then of group 1; r = 0..3]
+//   8 bits: the same with a 512-byte half tile per group: keys [token 4q+b: 8
+//          bytes; token 4q+b+2: 8 bytes], values [4 bytes of token 4q + r]
+//   scales: 8 bytes per token [key d0, d1, value d0, d1] at (2q + b) * 16 + c * 8
+//          for token 4q + b + 2c.
+// A 4-bit word holds element 2i in bits 4i and element 2i+1 in bits 16 + 4i; an
+// 8-bit word of 4 has the byte order 0, 2, 1, 3: masking (and shifting) a word
+// then gives pairs of neighbours in its two halves.
+#pragma once
+#include "common.cuh"
+
+namespace vla {
+namespace kv {
+
+constexpr int kPage = 64;  // tokens per page
+constexpr int HD = 64;
+constexpr int kTile = 16;
+
+template <int BITS>
+struct Block {
+  static constexpr int kTileCodes = kTile * HD * BITS / 8;      // bytes of a tile's key (or value) codes
+  static constexpr int kValues = kPage * HD * BITS / 8;         // offset of the value codes
+  static constexpr int kScales = 2 * kValues;                   // offset of the scales
+  static constexpr int kBytes = kScales + kPage * 8;            // 4608 or 8704
+};
+
+struct Cache {
+  uint8_t* pool;
+  const int* table;
+  long long table_ld;
+  int pages, max_pages, batch, kv_heads;
+};
+
+// Block of (sequence b, page slot, kv head); null, with the error recorded,
+// when the slot or the page number is out of range.
+template <int BITS>
+__device__ __forceinline__ uint8_t* block_of(const Cache& c, int b, int slot, int h) {
+  if (slot < 0 || slot >= c.max_pages) {
+    vla_record_error(VLA_DERR_KV_RANGE);
+    return nullptr;
+  }
+  const int page = c.table[(long long)b * c.table_ld + slot];
+  if (page < 0 || page >= c.pages) {
+    vla_record_error(VLA_DERR_KV_RANGE);
+    return nullptr;
+  }
+  return c.pool + ((long long)page * c.kv_heads + h) * Block<BITS>::kBytes;
+}
+
+// ---------------------------------------------------------------------------
+// word <-> numbers
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ __nv_bfloat162 as_bf2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32_t bits) { return (a & mask) | bits; }
+
+// The codes of a 4-bit word as bf16 pairs: 128 + n sits in the mantissa of
+// 0x4300 | n; subtracting 136 = 128 + 8 is exact.
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t* p) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    p[i] = as_u32(__hsub2(as_bf2(lop_and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u)), as_bf2(0x43084308u)));
+}
+
+// The codes of an 8-bit word (two's complement bytes) as two bf16 pairs: 128 +
+// the low seven bits, minus 128 or 256 by the sign bit (0x4380 is 256); exact.
+__device__ __forceinline__ void codes8(uint32_t w, uint32_t* p) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = w >> (8 * i);
+    p[i] = as_u32(__hsub2(as_bf2(lop_and_or(u, 0x007F007Fu, 0x43004300u)), as_bf2(lop_and_or(u, 0x00800080u, 0x43004300u))));
+  }
+}
+
+// Scale of a group from its largest positive and largest negative magnitude
+// (bf16 bits, the larger one >= 0).
+template <int BITS>
+__device__ __forceinline__ float group_scale(int hp, int hn) {
+  const int top = max(hp, hn);
+  const float a = __uint_as_float((uint32_t)top << 16);
+  float d;
+  if (BITS == 4) {
+    // a / 8 up to 5 significant bits: 4 of the 23 mantissa bits stay
+    d = __uint_as_float((__float_as_uint(a * 0.125f) + 0x0007FFFFu) & ~0x0007FFFFu);
+    d = fmaxf(d, 0x1p-100f);
+    if (hp > hn) d = -d;
+  } else {
+    // a in [2^k, 2^(k+1)): 127 * 2^(k-6) reaches it or 127 * 2^(k-5) does
+    const float p = __uint_as_float(__float_as_uint(a) & 0x7F800000u) * 0x1p-6f;
+    d = fmaxf(127.f * p >= a ? p : 2.f * p, 0x1p-100f);
+  }
+  return top >= 0x7F00 ? __uint_as_float(0x7FC00000u) : d;  // 0x7F00 is 2^127
+}
+
+// Codes of 8 elements with the scale's reciprocal r.
+// 4 bits: x r differs from x / d by less than 2^-20, while a quotient of an
+// 8-bit by a 5-bit significand that is no tie lies at least 2^-11 from every
+// half-integer within [-8.5, 8.5] (its distance is a multiple of 2^-5 / 62 when
+// it is near one at all).  The fused multiply-add onto 1.5 * 2^12 rounds to
+// multiples of 2^-11, which makes ties exact again and moves nothing else
+// across one; the second addition (1.5 * 2^23 + 8) rounds to integers, ties to
+// even, and leaves code + 8 in the low mantissa bits.
+__device__ __forceinline__ uint32_t pack4(const float* x, float r) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = fminf(fmaf(x[e], r, 6144.f) - 6144.f, 7.f);
+    const uint32_t n = __float_as_uint(q + 12582920.f) & 15u;
+    w |= n << (4 * (e >> 1) + 16 * (e & 1));
+  }
+  return w;
+}
+// 8 bits: d is a power of two, so x r is exact and one rounding does it.
+__device__ __forceinline__ uint32_t pack8(const float* x, float r) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t n = __float_as_uint(fmaf(x[e], r, 12582912.f)) & 255u;
+    w |= n << (16 * (e & 1) + 8 * (e >> 1));
+  }
+  return w;
+}
+
+// The largest positive and negative magnitudes of 8 bf16 (bits, as signed 16-bit
+// halves [positive | negative]) over the 4 lanes of a group.
+__device__ __forceinline__ uint32_t group_top(const uint4& u) {
+  const uint32_t f = 0x80008000u;
+  uint32_t hp = __vmaxs2(__vmaxs2(u.x, u.y), __vmaxs2(u.z, u.w));
+  uint32_t hn = __vmaxs2(__vmaxs2(u.x ^ f, u.y ^ f), __vmaxs2(u.z ^ f, u.w ^ f));
+  uint32_t m = __vmaxs2(__byte_perm(hp, hn, 0x5410), __byte_perm(hp, hn, 0x7632));  // low half: positive
+  m = __vmaxs2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  return __vmaxs2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+
+// Loads that keep nothing in L1: the cache and the rows are read once, and with
+// launch overlap an earlier kernel's line must not outlive the write between.
+__device__ __forceinline__ uint32_t ld_stream1(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_stream2(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+struct AppendParams {
+  Cache c;
+  const bf16* k;
+  const bf16* v;
+  long long k_row, v_row, k_batch, v_batch;
+  const int* start;
+  const int* count;  // valid tokens per sequence, or null
+  int n;             // tokens per sequence
+  int quads;         // aligned groups of 4 positions that n tokens can touch
+};
+
+// Coordinates of one warp's item: (sequence, quad of 4 cache positions, kv head).
+struct Item {
+  int b, h, token, slot, off;  // token: index of the lane's token among the n; off: position inside the page
+  bool live;
+};
+__device__ __forceinline__ Item item_of(long long w, int quads, int heads, int n, const int* start, const int* count,
+                                        int lane) {
+  Item it;
+  const int per = quads * heads;
+  it.b = (int)(w / per);
+  const int rem = (int)(w - (long long)it.b * per);
+  const int qd = rem / heads;
+  it.h = rem - qd * heads;
+  const int s = start != nullptr ? start[it.b] : 0;
+  const int valid = count != nullptr ? min(n, count[it.b]) : n;
+  const long long pos = (long long)((s >> 2) + qd) * 4 + (lane >> 3);
+  it.token = (int)(pos - s);
+  it.slot = (int)(pos / kPage);
+  it.off = (int)(pos % kPage);
+  it.live = it.token >= 0 && it.token < valid;
+  if (s < 0) {
+    vla_record_error(VLA_DERR_KV_RANGE);
+    it.live = false;
+  }
+  return it;
+}
+
+// One warp per (4 aligned cache positions, kv head): lane = (token r, 8 dims w).
+// It loads 16 bytes of K and of V per lane (each token's 128-byte row by 8
+// lanes), takes the scale over the 4 lanes of a group, and writes whole 128-byte
+// lines of codes (the order inside a tile keeps a quad's words together).
+template <int BITS>
+__global__ void __launch_bounds__(256) append_kernel(AppendParams p, long long items) {
+  pdl_prologue();
+  using B = Block<BITS>;
+  const long long warp = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (warp >= items) return;
+  const int lane = threadIdx.x & 31, w = lane & 7;
+  const Item it = item_of(warp, p.quads, p.c.kv_heads, p.n, p.start, p.count, lane);
+  uint4 x[2];
+  x[0] = x[1] = make_uint4(0u, 0u, 0u, 0u);
+  uint8_t* blk = nullptr;
+  if (it.live) {
+    const long long col = (long long)it.h * HD + w * 8;
+    x[0] = ld_stream(p.k + (long long)it.b * p.k_batch + (long long)it.token * p.k_row + col);
+    x[1] = ld_stream(p.v + (long long)it.b * p.v_batch + (long long)it.token * p.v_row + col);
+    blk = block_of<BITS>(p.c, it.b, it.slot, it.h);
+  }
+  const int tile = it.off >> 4, q = (it.off >> 2) & 3, r = it.off & 3, t = w & 3, grp = w >> 2;
+  uint32_t dd[2];  // scales (bf16 bits)
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {  // K, V
+    const uint32_t top = group_top(x[j]);
+    const float d = group_scale<BITS>((int)(short)(top & 0xFFFFu), (int)(short)(top >> 16));
+    dd[j] = __float_as_uint(d) >> 16;
+    float f[8];
+    unpack_bf16x8(x[j], f);
+    const float inv = 1.0f / d;
+    uint8_t* base = blk + (j == 0 ? 0 : B::kValues) + tile * B::kTileCodes;
+    if (BITS == 4) {
+      const uint32_t word = pack4(f, inv);
+      if (j == 0) {
+        if (blk) *reinterpret_cast<uint32_t*>(base + (2 * q + (r & 1)) * 64 + t * 16 + (r >> 1) * 8 + grp * 4) = word;
+      } else {
+        // a value word joins 4 dims of each group: swap halves with the other group's lane
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 4);
+        const uint32_t out = grp == 0 ? __byte_perm(word, other, 0x6240) : __byte_perm(other, word, 0x7351);
+        if (blk) *reinterpret_cast<uint32_t*>(base + q * 128 + (2 * t + grp) * 16 + r * 4) = out;
+      }
+    } else {
+      const uint32_t w0 = pack8(f, inv), w1 = pack8(f + 4, inv);
+      if (blk) {
+        base += grp * 512 + q * 128;
+        if (j == 0) {
+          *reinterpret_cast<uint2*>(base + (r & 1) * 64 + t * 16 + (r >> 1) * 8) = make_uint2(w0, w1);
+        } else {
+          *reinterpret_cast<uint32_t*>(base + (2 * t) * 16 + r * 4) = w0;
+          *reinterpret_cast<uint32_t*>(base + (2 * t + 1) * 16 + r * 4) = w1;
+        }
+      }
+    }
+  }
+  const uint32_t mine = dd[0] | dd[1] << 16;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 4);
+  if (blk && w == 0)
+    *reinterpret_cast<uint2*>(blk + B::kScales + tile * 128 + (2 * q + (r & 1)) * 16 + (r >> 1) * 8) =
+        make_uint2(__byte_perm(mine, other, 0x5410), __byte_perm(mine, other, 0x7632));
+}
+
+// ---------------------------------------------------------------------------
+// read back
+// ---------------------------------------------------------------------------
+struct ReadParams {
+  Cache c;
+  bf16* k;
+  bf16* v;
+  long long k_row, v_row, k_batch, v_batch;
+  const int* start;  // or null: 0
+  const int* count;  // valid tokens from start on per sequence, or null: n
+  int n, quads;
+};
+
+// The same mapping backwards; tokens past count are written as zeros.
+template <int BITS>
+__global__ void __launch_bounds__(256) read_kernel(ReadParams p, long long items) {
+  pdl_prologue();
+  using B = Block<BITS>;
+  const long long warp = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (warp >= items) return;
+  const int lane = threadIdx.x & 31, w = lane & 7;
+  const Item it = item_of(warp, p.quads, p.c.kv_heads, p.n, p.start, p.count, lane);
+  const uint8_t* blk = it.live ? block_of<BITS>(p.c, it.b, it.slot, it.h) : nullptr;
+  const int tile = it.off >> 4, q = (it.off >> 2) & 3, r = it.off & 3, t = w & 3, grp = w >> 2;
+  uint32_t a[2][2] = {{0u, 0u}, {0u, 0u}};
+  uint2 sc = make_uint2(0u, 0u);
+  if (blk) {
+    const uint8_t* kb = blk + tile * B::kTileCodes;
+    const uint8_t* vb = kb + B::kValues;
+    if (BITS == 4) {
+      a[0][0] = ld_stream1(kb + (2 * q + (r & 1)) * 64 + t * 16 + (r >> 1) * 8 + grp * 4);
+      a[1][0] = ld_stream1(vb + q * 128 + (2 * t + grp) * 16 + r * 4);
+    } else {
+      kb += grp * 512 + q * 128;
+      vb += grp * 512 + q * 128;
+      const uint2 u = ld_stream2(kb + (r & 1) * 64 + t * 16 + (r >> 1) * 8);
+      a[0][0] = u.x;
+      a[0][1] = u.y;
+      a[1][0] = ld_stream1(vb + (2 * t) * 16 + r * 4);
+      a[1][1] = ld_stream1(vb + (2 * t + 1) * 16 + r * 4);
+    }
+    sc = ld_stream2(blk + B::kScales + tile * 128 + (2 * q + (r & 1)) * 16 + (r >> 1) * 8);
+  }
+  if (BITS == 4) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, a[1][0], 4);
+    // group 0's words hold bytes 0 and 2, group 1's bytes 1 and 3 of both value words
+    a[1][0] = grp == 0 ? __byte_perm(a[1][0], other, 0x6240) : __byte_perm(other, a[1][0], 0x7351);
+  }
+  if (it.token < 0 || it.token >= p.n) return;
+  const long long col = (long long)it.h * HD + w * 8;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t o[4] = {0u, 0u, 0u, 0u};
+    if (blk) {
+      const uint32_t s2 = j == 0 ? sc.x : sc.y;
+      const __nv_bfloat162 d = as_bf2(__byte_perm(s2, s2, grp == 0 ? 0x1010 : 0x3232));
+      if (BITS == 4) {
+        codes4(a[j][0], o);
+      } else {
+        codes8(a[j][0], o);
+        codes8(a[j][1], o + 2);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = as_u32(__hmul2(as_bf2(o[i]), d));
+    }
+    bf16* dst = j == 0 ? p.k + (long long)it.b * p.k_batch + (long long)it.token * p.k_row + col
+                       : p.v + (long long)it.b * p.v_batch + (long long)it.token * p.v_row + col;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+}  // namespace kv
+}  // namespace vla

@@ -8,6 +8,7 @@
 #include "render.cuh"
 #include "gemm_host.cuh"
 #include "host_common.cuh"
+#include "kv_host.cuh"
 
 using namespace vla;
 
@@ -90,6 +91,8 @@ int vla_sync_check(void) {
   VLA_CUDA_TRY(cudaMemcpyFromSymbol(&code, g_vla_device_error, sizeof(code)));
   if (code != 0) {
     VLA_CUDA_TRY(cudaMemcpyToSymbol(g_vla_device_error, &zero, sizeof(zero)));
+    if (code == VLA_DERR_KV_RANGE)
+      return set_error(VLA_E_DEVICE_RANGE, "a cache position, length or page number was out of range (code 0x%x)", code);
     return set_error(VLA_E_DEVICE_TIMEOUT, "device wait limit expired (code 0x%x)", code);
   }
   return VLA_OK;
@@ -279,6 +282,27 @@ int vla_attention_bf16(const vla_attention_args* a, vla_stream_t stream) {
   p.scale_log2 = a->scale * 1.4426950408889634f;
   VLA_CHECK_ARG(a->impl >= VLA_ATTN_AUTO && a->impl <= VLA_ATTN_TCGEN05_PIPE, "attention: unknown impl %d", a->impl);
   return blocks::attention(p, a->batch, as_stream(stream), a->impl);
+}
+
+size_t vla_kv_block_bytes(int32_t bits) { return kv::block_bytes(bits); }
+
+int vla_kv_append_bf16(const vla_kv_cache* c, const void* k, int64_t k_row, int64_t k_batch, const void* v,
+                       int64_t v_row, int64_t v_batch, int32_t n, const int32_t* start, const int32_t* count,
+                       vla_stream_t stream) {
+  return kv::append(c, k, k_row, k_batch, v, v_row, v_batch, n, start, count, as_stream(stream));
+}
+
+int vla_kv_read_bf16(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, void* v, int64_t v_row,
+                     int64_t v_batch, int32_t n, const int32_t* start, const int32_t* count, vla_stream_t stream) {
+  return kv::read(c, k, k_row, k_batch, v, v_row, v_batch, n, start, count, as_stream(stream));
+}
+
+size_t vla_kv_attention_workspace(const vla_kv_cache* c, const vla_kv_attention_args* a) {
+  return kv::attention_workspace(c, a);
+}
+
+int vla_kv_attention_bf16(const vla_kv_cache* c, const vla_kv_attention_args* a, vla_stream_t stream) {
+  return kv::attention(c, a, as_stream(stream));
 }
 
 int vla_pixel_shuffle_bf16(const void* in, void* out, int32_t B, int32_t grid, int32_t scale, int32_t C,

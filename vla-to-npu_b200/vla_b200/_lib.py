@@ -19,6 +19,7 @@ VLA_E_CUDA = -3
 VLA_E_UNSUPPORTED = -4
 VLA_E_DEVICE_TIMEOUT = -5
 VLA_E_WORKSPACE = -6
+VLA_E_DEVICE_RANGE = -7
 
 ACT_NONE = 0
 ACT_GELU_TANH = 1
@@ -102,6 +103,32 @@ class VisionLayer(ctypes.Structure):
     ]
 
 
+class KVCacheDesc(ctypes.Structure):
+    """Mirror of ``vla_kv_cache``."""
+
+    _fields_ = [
+        ("pool", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_ld", ctypes.c_int64),
+        ("pages", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("batch", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("bits", ctypes.c_int32),
+    ]
+
+
+class KVAttentionArgs(ctypes.Structure):
+    """Mirror of ``vla_kv_attention_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("q_row", ctypes.c_int64), ("q_batch", ctypes.c_int64), ("o_row", ctypes.c_int64), ("o_batch", ctypes.c_int64),
+        ("lens", ctypes.c_void_p), ("q_len", ctypes.c_void_p),
+        ("Lq", ctypes.c_int32), ("Hq", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32), ("max_len", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+KV_PAGE = 64
+
+
 class ProfileRecord(ctypes.Structure):
     """Mirror of ``vla_profile_record``."""
 
@@ -142,6 +169,11 @@ SIGNATURES = {
     "vla_softmax_bf16": [_P, _I64, _P, _I64, _I64, _I64, _F32, _I32, _P],
     "vla_elementwise_bf16": [_I32, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P],
     "vla_attention_bf16": [ctypes.POINTER(AttentionArgs), _P],
+    "vla_kv_block_bytes": [_I32],
+    "vla_kv_append_bf16": [_P, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _P],
+    "vla_kv_read_bf16": [_P, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _P],
+    "vla_kv_attention_workspace": [_P, _P],
+    "vla_kv_attention_bf16": [_P, _P, _P],
     "vla_pixel_shuffle_bf16": [_P, _P, _I32, _I32, _I32, _I32, _P],
     "vla_patch_im2col_bf16": [_P, _P, _I32, _I32, _I32, _I32, _I32, _P],
     "vla_embed_bf16": [_P, _P, _I32, _I32, _I32, _I32, _F32, _P, _I64, _I32, _I32, _P],
@@ -158,7 +190,8 @@ SIGNATURES = {
     "vla_vision_layer_bf16": [ctypes.POINTER(VisionLayer), _P, _I32, _I32, _P, ctypes.c_size_t, _P],
 }
 _RET = {"vla_last_error": ctypes.c_char_p, "vla_launch_count": ctypes.c_uint64, "vla_llama_layer_workspace": ctypes.c_size_t,
-        "vla_vision_layer_workspace": ctypes.c_size_t, "vla_noalloc_scratch_bytes": ctypes.c_size_t}
+        "vla_vision_layer_workspace": ctypes.c_size_t, "vla_noalloc_scratch_bytes": ctypes.c_size_t,
+        "vla_kv_block_bytes": ctypes.c_size_t, "vla_kv_attention_workspace": ctypes.c_size_t}
 
 EW_GELU_TANH = 0
 EW_SILU = 1
