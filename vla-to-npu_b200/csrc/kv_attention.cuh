@@ -16,12 +16,15 @@
 // holds, and p d is selected to 0 where a key is not seen, so an unwritten or
 // masked slot's contents (NaN scales included) reach nothing.
 #pragma once
+#include <type_traits>
+
 #include "kvcache.cuh"
 
 namespace vla {
 namespace kv {
 
-constexpr int kUnit = 32;  // keys a warp takes at a time
+constexpr int kUnit = kPage;  // keys a warp takes at a time
+constexpr int kHalf = kUnit / 2;
 
 struct AttnParams {
   Cache c;
@@ -33,18 +36,20 @@ struct AttnParams {
   int Lq, Hq, G;
   int causal, window, sinks;
   float scale_log2;
+  uint32_t mask;     // code_mask<BITS>()
   int row_blocks;    // blocks of 8 * NT rows per (sequence, kv head)
   int parts, per;    // splits along the keys: units per part
   float* part_o;     // [(b, h, row block)][part][8 NT][64], when parts > 1
   float* part_ml;    // [...][8 NT][2]
 };
 
-// What a block of rows [r0, r0 + n) of one sequence sees: units [0, sink) and
+// What a block of rows [r0, r0 + n) of one sequence sees: units (pages) [0, sink) and
 // [first, last], numbered 0 .. count - 1.
 struct Span {
   int len, ql;    // keys, valid query tokens
   int lo, hi;     // positions of the first and last row's token
   int sink, first, count;
+  int open, shut, sink_open;  // units that every row sees whole: [open, shut) and [0, sink_open)
   int per;  // units of a part: the plan's, or more where the sequence is longer than the plan was made for
   __device__ __forceinline__ int unit(int u) const { return u < sink ? u : first + u - sink; }
   __device__ __forceinline__ int pos(int i, int causal) const { return causal ? len - ql + i : len - 1; }
@@ -62,10 +67,13 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int r0, int 
   const int i0 = r0 / p.G, i1 = min((r0 + n - 1) / p.G, s.ql - 1);
   s.lo = s.pos(i0, p.causal);
   s.hi = s.pos(i1, p.causal);
-  s.sink = s.first = s.count = 0;
+  s.sink = s.first = s.count = s.open = s.shut = s.sink_open = 0;
   s.per = p.per;
   if (i0 > i1 || s.hi < 0) return s;
+  s.shut = max(0, s.lo + 1) / kUnit;
   if (p.window > 0) {
+    s.open = (max(0, s.hi - p.window + 1) + kUnit - 1) / kUnit;
+    s.sink_open = min(p.sinks / kUnit, s.shut);
     s.first = max(0, s.lo - p.window + 1) / kUnit;
     s.sink = min((p.sinks + kUnit - 1) / kUnit, s.first);
   }
@@ -74,12 +82,17 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int r0, int 
   return s;
 }
 
-__device__ __forceinline__ void mma16n8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+// D = A B + C with C and D apart, so that a start value need not be copied.
+__device__ __forceinline__ void mma16n8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c0, float c1,
+                                        float c2, float c3) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void mma16n8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  mma16n8(d, a, b0, b1, d[0], d[1], d[2], d[3]);
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -92,43 +105,79 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// One unit's codes and scales in a lane's registers: two tiles of 16 keys.
-template <int BITS>
-struct UnitRegs {
-  uint4 k[2][BITS / 4], v[2][BITS / 4], s[2];
-};
-
-template <int BITS>
-__device__ __forceinline__ void load_unit(const uint8_t* blk, int half, int lane, UnitRegs<BITS>& u) {
-  using B = Block<BITS>;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int tile = 2 * half + i;
-    const uint8_t* kb = blk + tile * B::kTileCodes + lane * 16;
-    const uint8_t* vb = blk + B::kValues + tile * B::kTileCodes + (lane & 3) * 128 + (lane >> 2) * 16;
-#pragma unroll
-    for (int x = 0; x < BITS / 4; ++x) {
-      u.k[i][x] = ld_stream(kb + x * 512);
-      u.v[i][x] = ld_stream(vb + x * 512);
-    }
-    u.s[i] = ld_stream(blk + B::kScales + tile * 128 + (lane >> 2) * 16);
-  }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
-// The lane's operand registers of one tile's keys for the two groups of dims:
-// a[group][k-step][4] (rows g, g + 8; dims pairs).
+// Pages on their way through shared memory, one ring per warp; a stage is a page
+// in 4 bits and half of one in 8.  Keys and scales keep their order (a lane's 16
+// bytes lie at lane order); the 128-byte rows of the values (4 tokens) are 160
+// bytes apart, so that the eight lanes of a 16-byte access, 2 words of 4 rows,
+// touch all banks.
 template <int BITS>
-__device__ __forceinline__ void key_operand(const uint4* c, int grp, uint32_t (*a)[4]) {
+struct Ring {
+  static constexpr int kSteps = BITS == 4 ? 1 : 2;  // stages of a page
+  static constexpr int kTiles = 4 / kSteps;
+  static constexpr int kChunks = kTiles * BITS / 4;  // 512-byte pieces of a stage's keys (or values)
+  static constexpr int kVOff = kChunks * 512;
+  static constexpr int kSOff = kVOff + kChunks * 640;
+  static constexpr int kStage = kSOff + kTiles * 128;  // 5120 or 4864 bytes
+  static constexpr int kStages = BITS == 4 ? 2 : 3;
+  static constexpr int kWarpBytes = kStage * kStages;
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+
+template <int BITS>
+__device__ __forceinline__ void copy_stage(uint32_t stage, const uint8_t* blk, int step, int lane) {
+  using B = Block<BITS>;
+  using Rg = Ring<BITS>;
+  const uint8_t* src = blk + step * (Rg::kChunks * 512) + lane * 16;
+  const uint32_t vdst = stage + Rg::kVOff + (lane >> 3) * 160 + (lane & 7) * 16;
+#pragma unroll
+  for (int i = 0; i < Rg::kChunks; ++i) {
+    copy16(stage + i * 512 + lane * 16, src + i * 512);
+    copy16(vdst + i * 640, src + B::kValues + i * 512);
+  }
+  if (Rg::kTiles == 4 || lane < 16)
+    copy16(stage + Rg::kSOff + lane * 16, blk + B::kScales + step * (Rg::kTiles * 128) + lane * 16);
+}
+
+// The lane's operand registers of one tile's keys and one group of dims:
+// a[k-step][4] (rows g, g + 8; dims pairs).  4-bit codes stay 136 too large
+// (128 + n instead of code = n - 8): the product starts from -136 sum(q)
+// instead, which spares the subtractions; the sums' rounding, 2^-24 of
+// 136 |sum q|, stays far below bf16's 2^-8 in the probabilities.
+template <int BITS>
+__device__ __forceinline__ void key_operand(const uint4* c, int grp, uint32_t mask, uint32_t (*a)[4]) {
   uint32_t lo[4], hi[4];  // token 4q+b (row g), token 4q+b+2 (row g + 8)
   if (BITS == 4) {
-    codes4(grp == 0 ? c[0].x : c[0].y, lo);
-    codes4(grp == 0 ? c[0].z : c[0].w, hi);
+    const uint32_t wl = grp == 0 ? c[0].x : c[0].y, wh = grp == 0 ? c[0].z : c[0].w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = lop_and_or(wl >> (4 * i), mask, 0x43004300u);
+      hi[i] = lop_and_or(wh >> (4 * i), mask, 0x43004300u);
+    }
   } else {
     const uint4 w = c[grp];
-    codes8(w.x, lo);
-    codes8(w.y, lo + 2);
-    codes8(w.z, hi);
-    codes8(w.w, hi + 2);
+    codes8(w.x, mask, lo);
+    codes8(w.y, mask, lo + 2);
+    codes8(w.z, mask, hi);
+    codes8(w.w, mask, hi + 2);
   }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -142,7 +191,7 @@ __device__ __forceinline__ void key_operand(const uint4* c, int grp, uint32_t (*
 // The lane's operand registers of one tile's values, group grp: two 16-dim
 // pieces m (rows: dims 4g + 2m and 4g + 2m + 1; columns: tokens 4t .. 4t+3).
 template <int BITS>
-__device__ __forceinline__ void value_operand(const uint4* c, int grp, uint32_t (*a)[4]) {
+__device__ __forceinline__ void value_operand(const uint4* c, int grp, uint32_t mask, uint32_t (*a)[4]) {
   const uint4 w = c[BITS == 4 ? 0 : grp];
   const uint32_t e01 = __byte_perm(w.x, w.y, 0x5410), o01 = __byte_perm(w.x, w.y, 0x7632);
   const uint32_t e23 = __byte_perm(w.z, w.w, 0x5410), o23 = __byte_perm(w.z, w.w, 0x7632);
@@ -150,18 +199,18 @@ __device__ __forceinline__ void value_operand(const uint4* c, int grp, uint32_t 
   for (int m = 0; m < 2; ++m) {
     if (BITS == 4) {
       const int sh = 8 * grp + 4 * m;
-      a[m][0] = as_u32(__hsub2(as_bf2(lop_and_or(e01 >> sh, 0x000F000Fu, 0x43004300u)), as_bf2(0x43084308u)));
-      a[m][1] = as_u32(__hsub2(as_bf2(lop_and_or(o01 >> sh, 0x000F000Fu, 0x43004300u)), as_bf2(0x43084308u)));
-      a[m][2] = as_u32(__hsub2(as_bf2(lop_and_or(e23 >> sh, 0x000F000Fu, 0x43004300u)), as_bf2(0x43084308u)));
-      a[m][3] = as_u32(__hsub2(as_bf2(lop_and_or(o23 >> sh, 0x000F000Fu, 0x43004300u)), as_bf2(0x43084308u)));
+      a[m][0] = as_u32(__hsub2(as_bf2(lop_and_or(e01 >> sh, mask, 0x43004300u)), as_bf2(0x43084308u)));
+      a[m][1] = as_u32(__hsub2(as_bf2(lop_and_or(o01 >> sh, mask, 0x43004300u)), as_bf2(0x43084308u)));
+      a[m][2] = as_u32(__hsub2(as_bf2(lop_and_or(e23 >> sh, mask, 0x43004300u)), as_bf2(0x43084308u)));
+      a[m][3] = as_u32(__hsub2(as_bf2(lop_and_or(o23 >> sh, mask, 0x43004300u)), as_bf2(0x43084308u)));
     }
   }
   if (BITS == 8) {
     uint32_t x[4][2];
-    codes8(e01, x[0]);
-    codes8(o01, x[1]);
-    codes8(e23, x[2]);
-    codes8(o23, x[3]);
+    codes8(e01, mask, x[0]);
+    codes8(o01, mask, x[1]);
+    codes8(e23, mask, x[2]);
+    codes8(o23, mask, x[3]);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
 #pragma unroll
@@ -171,16 +220,22 @@ __device__ __forceinline__ void value_operand(const uint4* c, int grp, uint32_t 
 }
 
 constexpr int kWarps = 4;
+template <int BITS, int NT>
+constexpr int attend_smem() {
+  const int rings = kWarps * Ring<BITS>::kWarpBytes, join = kWarps * 8 * NT * (HD + 4 + 2) * (int)sizeof(float);
+  return rings > join ? rings : join;
+}
 
 // One CTA per (part, kv head, row block, sequence): its warps take the part's
 // units in turn, each with its own running maximum, sum and output, which are
-// joined in shared memory at the end.
+// joined in shared memory at the end.  A warp copies half pages into its own ring
+// ahead of its computation (cp.async; no warp waits for another).
 template <int BITS, int NT>
 __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   pdl_prologue();
   constexpr int R = 8 * NT;
-  __shared__ float sO[kWarps][R][HD + 4];
-  __shared__ float sM[kWarps][R], sL[kWarps][R];
+  using Rg = Ring<BITS>;
+  extern __shared__ __align__(128) uint8_t smem[];  // the rings; after the loop the warps' results
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   int x = blockIdx.x;  // kv head, part, row block, sequence
   const int h = x % p.c.kv_heads;
@@ -193,9 +248,42 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   const int u0 = part * sp.per, u1 = min(sp.count, u0 + sp.per);
   if (part > 0 && u0 >= sp.count) return;  // part 0 writes the rows that see nothing
 
+  const int* table = p.c.table + (long long)b * p.c.table_ld;
+  auto page_of = [&](int u) { return u < u1 ? table[sp.unit(u)] : 0; };  // slots lie inside the table (span_of)
+  auto block = [&](int u, int page) -> const uint8_t* {
+    if (u >= u1) return nullptr;
+    if (page < 0 || page >= p.c.pages) {
+      vla_record_error(VLA_DERR_KV_RANGE);
+      return nullptr;
+    }
+    return p.c.pool + ((long long)page * p.c.kv_heads + h) * Block<BITS>::kBytes;
+  };
+  const int steps = u0 + warp < u1 ? Rg::kSteps * ((u1 - u0 - warp + kWarps - 1) / kWarps) : 0;
+  const uint32_t ring = smem_u32(smem) + warp * Rg::kWarpBytes;
+  int iu = u0 + warp, page = page_of(iu), next = 0, put = 0;  // copies: unit, page number, step, stage
+  const uint8_t* blk = nullptr;
+  uint32_t valid = 0;  // stages that hold (a part of) a page that exists
+  auto issue = [&]() {
+    if (next < steps) {
+      if (Rg::kSteps == 1 || (next & 1) == 0) {
+        blk = block(iu, page);
+        iu += kWarps;
+        page = page_of(iu);
+      }
+      valid = blk ? valid | (1u << put) : valid & ~(1u << put);
+      if (blk) copy_stage<BITS>(ring + put * Rg::kStage, blk, next % Rg::kSteps, lane);
+    }
+    copy_commit();
+    ++next;
+    put = put == Rg::kStages - 1 ? 0 : put + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < Rg::kStages - 1; ++i) issue();
+
   // query operand: column g of n-tile j is row r0 + 8j + g, dims 32 grp + 8t .. + 7
   uint32_t qf[NT][2][4];
   int pos[NT][2];  // positions of the accumulator's columns 2t, 2t + 1
+  float2 init[NT][2];  // what the columns' partial products start from
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int r = r0 + 8 * j + g;
@@ -209,6 +297,16 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
       qf[j][grp][1] = x.y;
       qf[j][grp][2] = x.z;
       qf[j][grp][3] = x.w;
+      init[j][grp] = make_float2(0.f, 0.f);
+      if (BITS == 4) {
+        float f[8];
+        unpack_bf16x8(x, f);
+        float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        init[j][grp].x = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t);
+        init[j][grp].y = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      }
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -218,153 +316,176 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   }
 
   float o[NT][4][4];
-  float m[NT][2], l[NT][2];
+  float m[NT][2];       // running maxima of the columns (raw products)
+  float2 l[NT], ms[NT]; // sums of the lane's keys; -m * scale log2(e), 0 while there is no maximum
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
     m[j][0] = m[j][1] = -INFINITY;
-    l[j][0] = l[j][1] = 0.f;
+    l[j] = ms[j] = make_float2(0.f, 0.f);
   }
   const float grow = 8.f / p.scale_log2;  // the maximum moves in steps above 2^8 only
+  const uint32_t mask = p.mask;
+  const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
 
-  auto block = [&](int u) -> const uint8_t* {
-    return u < u1 ? block_of<BITS>(p.c, b, sp.unit(u) >> 1, h) : nullptr;
-  };
-  UnitRegs<BITS> cur;
-  const uint8_t* blk = block(u0 + warp);
-  if (blk) load_unit<BITS>(blk, sp.unit(u0 + warp) & 1, lane, cur);
-#pragma unroll 1
-  for (int u = u0 + warp; u < u1; u += kWarps) {
-    const uint8_t* nblk = block(u + kWarps);
-    UnitRegs<BITS> nxt;
-    if (nblk) load_unit<BITS>(nblk, sp.unit(u + kWarps) & 1, lane, nxt);
-    if (blk) {
-      const int key0 = sp.unit(u) * kUnit;
-      float s[2][NT][4];
+  auto compute = [&](uint32_t stage, int half, int key0, auto masked) {  // 32 keys
+    constexpr bool MASK = decltype(masked)::value;
+    const uint32_t ka = stage + half * (BITS * 256) + lane * 16;
+    const uint32_t va = stage + Rg::kVOff + half * (BITS * 320) + t * 160 + g * 16;
+    const uint32_t sa = stage + Rg::kSOff + half * 256 + g * 16;
+    uint4 sc[2];
+    sc[0] = lds16(sa);
+    sc[1] = lds16(sa + 128);
+    float2 s[2][NT][2];  // [tile][n-tile][key g or g + 8] over the columns 2t, 2t + 1
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float s1[NT][4];
-        uint32_t a[2][4];
+    for (int i = 0; i < 2; ++i) {
+      float s0[NT][4], s1[NT][4];
+      uint32_t a[2][4];
+      uint4 kc[BITS / 4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][j][e] = s1[j][e] = 0.f;
-        }
-        key_operand<BITS>(cur.k[i], 0, a);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          mma16n8(s[i][j], a[0], qf[j][0][0], qf[j][0][1]);
-          mma16n8(s[i][j], a[1], qf[j][0][2], qf[j][0][3]);
-        }
-        key_operand<BITS>(cur.k[i], 1, a);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          mma16n8(s1[j], a[0], qf[j][1][0], qf[j][1][1]);
-          mma16n8(s1[j], a[1], qf[j][1][2], qf[j][1][3]);
-        }
-        const float da0 = __uint_as_float(cur.s[i].x << 16), da1 = __uint_as_float(cur.s[i].x & 0xFFFF0000u);
-        const float db0 = __uint_as_float(cur.s[i].z << 16), db1 = __uint_as_float(cur.s[i].z & 0xFFFF0000u);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          s[i][j][0] = fmaf(s[i][j][0], da0, s1[j][0] * da1);
-          s[i][j][1] = fmaf(s[i][j][1], da0, s1[j][1] * da1);
-          s[i][j][2] = fmaf(s[i][j][2], db0, s1[j][2] * db1);
-          s[i][j][3] = fmaf(s[i][j][3], db0, s1[j][3] * db1);
-        }
-      }
-      // keys that a row does not see; `seen` bit (i, j, e)
-      const bool inside = key0 + kUnit - 1 <= sp.lo &&
-                          (p.window <= 0 || key0 > sp.hi - p.window || key0 + kUnit <= p.sinks);
-      uint32_t hidden[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) hidden[j] = 0u;
-      if (!inside) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int ka = key0 + i * 16 + 4 * (g >> 1) + (g & 1);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = ka + (e & 2), at = pos[j][e & 1];
-              const bool sees = key <= at && (p.window <= 0 || key > at - p.window || key < p.sinks);
-              if (!sees) {
-                hidden[j] |= 1u << (4 * i + e);
-                s[i][j][e] = -INFINITY;
-              }
-            }
-          }
-        }
-      }
-      bool moves = false;
+      for (int c = 0; c < BITS / 4; ++c) kc[c] = lds16(ka + (i * (BITS / 4) + c) * 512);
+      key_operand<BITS>(kc, 0, mask, a);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float top = fmaxf(fmaxf(s[0][j][c], s[0][j][c + 2]), fmaxf(s[1][j][c], s[1][j][c + 2]));
-          moves |= top > m[j][c] + grow || (m[j][c] == -INFINITY && top > -INFINITY);
-        }
+        mma16n8(s0[j], a[0], qf[j][0][0], qf[j][0][1], init[j][0].x, init[j][0].y, init[j][0].x, init[j][0].y);
+        mma16n8(s0[j], a[1], qf[j][0][2], qf[j][0][3]);
       }
-      if (__any_sync(0xffffffffu, moves)) {
+      key_operand<BITS>(kc, 1, mask, a);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(fmaxf(s[0][j][c], s[0][j][c + 2]), fmaxf(s[1][j][c], s[1][j][c + 2]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float to = fmaxf(m[j][c], top);
-            const float f = to == m[j][c] ? 1.f : ex2((m[j][c] - to) * p.scale_log2);
-            m[j][c] = to;
-            l[j][c] *= f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              o[j][i][c] *= f;
-              o[j][i][c + 2] *= f;
-            }
-          }
-        }
+      for (int j = 0; j < NT; ++j) {
+        mma16n8(s1[j], a[0], qf[j][1][0], qf[j][1][1], init[j][1].x, init[j][1].y, init[j][1].x, init[j][1].y);
+        mma16n8(s1[j], a[1], qf[j][1][2], qf[j][1][3]);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t b0[NT][2], b1[NT][2];
-        const float va0 = __uint_as_float(cur.s[i].y << 16), va1 = __uint_as_float(cur.s[i].y & 0xFFFF0000u);
-        const float vb0 = __uint_as_float(cur.s[i].w << 16), vb1 = __uint_as_float(cur.s[i].w & 0xFFFF0000u);
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t d = k == 0 ? sc[i].x : sc[i].z;
+        const float d0 = __uint_as_float(d << 16), d1 = __uint_as_float(d & 0xFFFF0000u);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          float e[4], x0[4], x1[4];
+        for (int j = 0; j < NT; ++j)
+          s[i][j][k] = __ffma2_rn(make_float2(s0[j][2 * k], s0[j][2 * k + 1]), make_float2(d0, d0),
+                                  __fmul2_rn(make_float2(s1[j][2 * k], s1[j][2 * k + 1]), make_float2(d1, d1)));
+      }
+    }
+    uint32_t hidden[NT];
+    if (MASK) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float mc = m[j][c & 1];
-            e[c] = ex2(fmaf(s[i][j][c], p.scale_log2, mc == -INFINITY ? 0.f : -mc * p.scale_log2));
-            const bool off = (hidden[j] >> (4 * i + c)) & 1u;
-            l[j][c & 1] += e[c];
-            x0[c] = off ? 0.f : e[c] * (c < 2 ? va0 : vb0);
-            x1[c] = off ? 0.f : e[c] * (c < 2 ? va1 : vb1);
-          }
-          // P^T rounded to bf16 with its value scales (2^-9 of each term, as bf16 values have)
-          b0[j][0] = transpose8(pack_bf16x2(x0[0], x0[1]));
-          b1[j][0] = transpose8(pack_bf16x2(x0[2], x0[3]));
-          b0[j][1] = transpose8(pack_bf16x2(x1[0], x1[1]));
-          b1[j][1] = transpose8(pack_bf16x2(x1[2], x1[3]));
-        }
+      for (int j = 0; j < NT; ++j) {
+        hidden[j] = 0u;
 #pragma unroll
-        for (int grp = 0; grp < 2; ++grp) {
-          uint32_t a[2][4];
-          value_operand<BITS>(cur.v[i], grp, a);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            mma16n8(o[j][2 * grp], a[0], b0[j][grp], b1[j][grp]);
-            mma16n8(o[j][2 * grp + 1], a[1], b0[j][grp], b1[j][grp]);
+        for (int e = 0; e < 8; ++e) {
+          const int i = e >> 2, k = (e >> 1) & 1, c = e & 1;
+          const int key = key0 + i * 16 + 4 * (g >> 1) + (g & 1) + 2 * k, at = pos[j][c];
+          if (key > at || (p.window > 0 && key <= at - p.window && key >= p.sinks)) {
+            hidden[j] |= 1u << e;
+            (c == 0 ? s[i][j][k].x : s[i][j][k].y) = -INFINITY;
           }
         }
       }
     }
-    cur = nxt;
-    blk = nblk;
+    bool moves = false;
+    float2 top[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      top[j].x = max3(s[0][j][0].x, s[0][j][1].x, fmaxf(s[1][j][0].x, s[1][j][1].x));
+      top[j].y = max3(s[0][j][0].y, s[0][j][1].y, fmaxf(s[1][j][0].y, s[1][j][1].y));
+      // (from no maximum, -inf + grow is -inf and any score moves it)
+      moves |= top[j].x > m[j][0] + grow || top[j].y > m[j][1] + grow;
+    }
+    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float tp = c == 0 ? top[j].x : top[j].y;
+          tp = fmaxf(tp, __shfl_xor_sync(0xffffffffu, tp, 4));
+          tp = fmaxf(tp, __shfl_xor_sync(0xffffffffu, tp, 8));
+          tp = fmaxf(tp, __shfl_xor_sync(0xffffffffu, tp, 16));
+          const float to = fmaxf(m[j][c], tp);
+          const float f = to == m[j][c] ? 1.f : ex2((m[j][c] - to) * p.scale_log2);
+          m[j][c] = to;
+          const float neg = to == -INFINITY ? 0.f : -to * p.scale_log2;
+          if (c == 0) {
+            ms[j].x = neg;
+            l[j].x *= f;
+          } else {
+            ms[j].y = neg;
+            l[j].y *= f;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[j][i][c] *= f;
+            o[j][i][c + 2] *= f;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint4 vc[BITS / 4];
+#pragma unroll
+      for (int c = 0; c < BITS / 4; ++c) vc[c] = lds16(va + (i * (BITS / 4) + c) * 640);
+      uint32_t pt[NT][2][2];  // P^T operand [n-tile][group][key half]
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t d = k == 0 ? sc[i].y : sc[i].w;
+        const float d0 = __uint_as_float(d << 16), d1 = __uint_as_float(d & 0xFFFF0000u);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float2 e = __ffma2_rn(s[i][j][k], sl2, ms[j]);
+          e.x = ex2(e.x);
+          e.y = ex2(e.y);
+          l[j] = __fadd2_rn(l[j], e);
+          float2 x0 = __fmul2_rn(e, make_float2(d0, d0)), x1 = __fmul2_rn(e, make_float2(d1, d1));
+          if (MASK) {  // 0 times a scale that is NaN
+            if ((hidden[j] >> (4 * i + 2 * k)) & 1u) x0.x = x1.x = 0.f;
+            if ((hidden[j] >> (4 * i + 2 * k)) & 2u) x0.y = x1.y = 0.f;
+          }
+          // P^T rounded to bf16 with its value scales (2^-8 of each term, as bf16 values have)
+          pt[j][0][k] = transpose8(pack_bf16x2(x0.x, x0.y));
+          pt[j][1][k] = transpose8(pack_bf16x2(x1.x, x1.y));
+        }
+      }
+#pragma unroll
+      for (int grp = 0; grp < 2; ++grp) {
+        uint32_t a[2][4];
+        value_operand<BITS>(vc, grp, mask, a);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          mma16n8(o[j][2 * grp], a[0], pt[j][grp][0], pt[j][grp][1]);
+          mma16n8(o[j][2 * grp + 1], a[1], pt[j][grp][0], pt[j][grp][1]);
+        }
+      }
+    }
+  };
+
+  int get = 0;
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    issue();
+    copy_wait<Rg::kStages - 1>();
+    __syncwarp();
+    const int un = sp.unit(u0 + warp + i / Rg::kSteps * kWarps);
+    if ((valid >> get) & 1u) {
+      const uint32_t stage = ring + get * Rg::kStage;
+      int key0 = un * kUnit + i % Rg::kSteps * kHalf;
+      if ((un >= sp.open && un < sp.shut) || un < sp.sink_open) {
+#pragma unroll
+        for (int half = 0; half < 2 / Rg::kSteps; ++half) compute(stage, half, key0 + half * kHalf, std::false_type());
+      } else {
+#pragma unroll 1
+        for (int half = 0; half < 2 / Rg::kSteps; ++half, key0 += kHalf)
+          if (key0 <= sp.hi) compute(stage, half, key0, std::true_type());
+      }
+    }
+    __syncwarp();
+    get = get == Rg::kStages - 1 ? 0 : get + 1;
   }
+  copy_wait<0>();
+  __syncthreads();  // the rings' memory is free
+  float(*sO)[R][HD + 4] = reinterpret_cast<float(*)[R][HD + 4]>(smem);
+  float(*sM)[R] = reinterpret_cast<float(*)[R]>(smem + sizeof(float) * kWarps * R * (HD + 4));
+  float(*sL)[R] = sM + kWarps;
 
   // join the warps: columns 2t, 2t+1 of n-tile j are rows 8j + 2t (+ 1); piece
   // 2 grp + n holds dims 32 grp + 4g + 2n and that + 1
@@ -372,7 +493,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   for (int j = 0; j < NT; ++j) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float sum = l[j][c];
+      float sum = c == 0 ? l[j].x : l[j].y;
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
@@ -422,40 +543,56 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   }
 }
 
-// Joins the parts of a block of rows in their order: one warp per row, two dims
-// per lane.
+// Joins the parts of a row, in an order that their number alone sets: one CTA
+// per row of a kv head, each warp a share of the parts, two dims per lane.
+constexpr int kJoinWarps = 8;
 template <int NT>
-__global__ void __launch_bounds__(256) join_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p) {
   pdl_prologue();
   constexpr int R = 8 * NT;
-  int x = blockIdx.x;
-  const int h = x % p.c.kv_heads;
-  x /= p.c.kv_heads;
-  const int rb = x % p.row_blocks, b = x / p.row_blocks;
-  const int rows = p.Lq * p.G, r0 = rb * R;
-  const Span sp = span_of(p, b, r0, R);
+  __shared__ float sO[kJoinWarps][HD];
+  __shared__ float sL[kJoinWarps];
+  const int rows = p.Lq * p.G;
+  const long long hb = blockIdx.x / rows;  // kv head, sequence
+  const int row = (int)(blockIdx.x - hb * rows);
+  const int h = (int)(hb % p.c.kv_heads), b = (int)(hb / p.c.kv_heads);
+  const int rb = row / R, r = row - rb * R, i = row / p.G, head = h * p.G + row - i * p.G;
+  const Span sp = span_of(p, b, rb * R, R);
   if (sp.count <= sp.per) return;  // written whole
   const int n = (sp.count + sp.per - 1) / sp.per;
-  const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < R && r0 + r < rows; r += 8) {
-    const int row = r0 + r, i = row / p.G, head = h * p.G + row - i * p.G;
-    const long long slot = (((long long)b * p.row_blocks + rb) * p.c.kv_heads + h) * p.parts;
-    float top = -INFINITY;
-    for (int y = 0; y < n; ++y) top = fmaxf(top, p.part_ml[((slot + y) * R + r) * 2]);
-    float sum = 0.f, a0 = 0.f, a1 = 0.f;
-    for (int y = 0; y < n; ++y) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + ((slot + y) * R + r) * 2);
-      const float f = ml.x == -INFINITY ? 0.f : ex2((ml.x - top) * p.scale_log2);
-      const float2 v = *reinterpret_cast<const float2*>(p.part_o + ((slot + y) * R + r) * HD + 2 * lane);
-      sum += ml.x == -INFINITY ? ml.y : f * ml.y;
-      a0 += f * v.x;
-      a1 += f * v.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long slot = (((long long)b * p.row_blocks + rb) * p.c.kv_heads + h) * p.parts;
+  const float* ml = p.part_ml + (slot * R + r) * 2;
+  const float* po = p.part_o + (slot * R + r) * HD + 2 * lane;
+  float top = -INFINITY;
+  for (int y = lane; y < n; y += 32) top = fmaxf(top, ml[(long long)y * (2 * R)]);
+  top = warp_max(top);
+  float sum = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll 4
+  for (int y = warp; y < n; y += kJoinWarps) {
+    const float2 v = *reinterpret_cast<const float2*>(po + (long long)y * (R * HD));
+    const float2 w = *reinterpret_cast<const float2*>(ml + (long long)y * (2 * R));
+    const float f = w.x == -INFINITY ? 0.f : ex2((w.x - top) * p.scale_log2);
+    sum += w.x == -INFINITY ? w.y : f * w.y;
+    a0 += f * v.x;
+    a1 += f * v.y;
+  }
+  sO[warp][2 * lane] = a0;
+  sO[warp][2 * lane + 1] = a1;
+  if (lane == 0) sL[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    sum = a0 = a1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      sum += sL[w];
+      a0 += sO[w][2 * lane];
+      a1 += sO[w][2 * lane + 1];
     }
     const bool empty = i >= sp.ql || sum == 0.f;
     const float inv = empty ? 0.f : 1.f / sum;
-    const uint32_t out = empty ? 0u : pack_bf16x2(a0 * inv, a1 * inv);
     *reinterpret_cast<uint32_t*>(p.o + (long long)b * p.o_batch + (long long)i * p.o_row + (long long)head * HD +
-                                 2 * lane) = out;
+                                 2 * lane) = empty ? 0u : pack_bf16x2(a0 * inv, a1 * inv);
   }
 }
 

@@ -105,14 +105,16 @@ static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a,
   const long long room = (long long)c->max_pages * kPage;
   long long keys = a->max_len > 0 && a->max_len < room ? a->max_len : room;
   if (a->window > 0) {
-    // the window of a block's rows and the first tokens, at 32-key granularity
+    // the window of a block's rows and the first tokens, in whole pages
     const long long seen = (long long)a->window + a->sinks + (8 * out->nt - 1) / (a->Hq / c->kv_heads) + 3 * kUnit;
     if (seen < keys) keys = seen;
   }
   const long long units = (keys + kUnit - 1) / kUnit;
   const long long base = (long long)c->batch * c->kv_heads * out->row_blocks;
-  const long long want = (12ll * device_info().num_sms + base - 1) / base;
-  const long long most = (units + 15) / 16;
+  static const int per_sm = []() { const char* e = getenv("KV_PER_SM"); return e ? atoi(e) : 12; }();
+  static const int min_units = []() { const char* e = getenv("KV_MIN_UNITS"); return e ? atoi(e) : 8; }();
+  const long long want = ((long long)per_sm * device_info().num_sms + base - 1) / base;
+  const long long most = (units + min_units - 1) / min_units;
   long long parts = want < most ? want : most;
   if (parts < 1) parts = 1;
   out->per = (int)((units + parts - 1) / parts);
@@ -134,10 +136,15 @@ static int check_attention(const vla_kv_cache* c, const vla_kv_attention_args* a
 }
 
 template <int BITS, int NT>
-static void launch_attend(const AttnParams& p, const Plan& pl, cudaStream_t st) {
+static int launch_attend(const AttnParams& p, const Plan& pl, cudaStream_t st) {
+  constexpr int smem = attend_smem<BITS, NT>();
+  VLA_CUDA_TRY(cudaFuncSetAttribute(attend_kernel<BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const long long base = (long long)p.c.batch * p.c.kv_heads * pl.row_blocks;
-  launch_k(attend_kernel<BITS, NT>, dim3((unsigned)(base * pl.parts)), dim3(kWarps * 32), 0, st, p);
-  if (pl.parts > 1) launch_k(join_kernel<NT>, dim3((unsigned)base), dim3(256), 0, st, p);
+  launch_k(attend_kernel<BITS, NT>, dim3((unsigned)(base * pl.parts)), dim3(kWarps * 32), smem, st, p);
+  if (pl.parts > 1)
+    launch_k(join_kernel<NT>, dim3((unsigned)((long long)p.c.batch * p.c.kv_heads * p.Lq * p.G)), dim3(kJoinWarps * 32),
+             0, st, p);
+  return VLA_OK;
 }
 
 static size_t attention_workspace(const vla_kv_cache* c, const vla_kv_attention_args* a) {
@@ -179,26 +186,29 @@ static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cuda
   p.window = a->window > 0 && a->window < room ? a->window : 0;
   p.sinks = a->sinks < room ? a->sinks : (int)room;
   p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.mask = c->bits == 4 ? code_mask<4>() : code_mask<8>();
   p.row_blocks = pl.row_blocks;
   p.parts = pl.parts;
   p.per = pl.per;
   p.part_o = (float*)a->workspace;
   if (pl.parts > 1)
     p.part_ml = p.part_o + (size_t)c->batch * c->kv_heads * pl.row_blocks * pl.parts * 8 * pl.nt * HD;
+  int rc;
   prof_begin(st);
   if (c->bits == 4) {
-    if (pl.nt == 1) launch_attend<4, 1>(p, pl, st);
-    else if (pl.nt == 2) launch_attend<4, 2>(p, pl, st);
-    else launch_attend<4, 4>(p, pl, st);
+    if (pl.nt == 1) rc = launch_attend<4, 1>(p, pl, st);
+    else if (pl.nt == 2) rc = launch_attend<4, 2>(p, pl, st);
+    else rc = launch_attend<4, 4>(p, pl, st);
   } else {
-    if (pl.nt == 1) launch_attend<8, 1>(p, pl, st);
-    else if (pl.nt == 2) launch_attend<8, 2>(p, pl, st);
-    else launch_attend<8, 4>(p, pl, st);
+    if (pl.nt == 1) rc = launch_attend<8, 1>(p, pl, st);
+    else if (pl.nt == 2) rc = launch_attend<8, 2>(p, pl, st);
+    else rc = launch_attend<8, 4>(p, pl, st);
   }
   // the lengths are on the device: the profile counts whole caches (or windows)
   const double keys = (double)pl.per * pl.parts * kUnit;
   prof_end(st, VLA_KIND_ATTENTION, 4.0 * c->batch * a->Hq * (double)a->Lq * keys * HD,
            c->batch * (keys * c->kv_heads * block_bytes(c->bits) / kPage + 4.0 * a->Lq * a->Hq * HD));
+  VLA_TRY(rc);
   return launch_status("kv_attention");
 }
 

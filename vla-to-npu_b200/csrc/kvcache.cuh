@@ -83,23 +83,36 @@ __device__ __forceinline__ uint8_t* block_of(const Cache& c, int b, int slot, in
 __device__ __forceinline__ __nv_bfloat162 as_bf2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32_t bits) { return (a & mask) | bits; }
+// (a & mask) | bits in one instruction.  It takes one immediate only, so a mask
+// that is a constant to the compiler costs a second one: the attention kernel
+// passes it as a launch argument.
+__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(bits));
+  return d;
+}
+
+// mask selects a code's magnitude bits in both halves: the low ones of a code.
+template <int BITS>
+constexpr uint32_t code_mask() {
+  return BITS == 4 ? 0x000F000Fu : 0x007F007Fu;
+}
 
 // The codes of a 4-bit word as bf16 pairs: 128 + n sits in the mantissa of
 // 0x4300 | n; subtracting 136 = 128 + 8 is exact.
-__device__ __forceinline__ void codes4(uint32_t w, uint32_t* p) {
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t mask, uint32_t* p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    p[i] = as_u32(__hsub2(as_bf2(lop_and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u)), as_bf2(0x43084308u)));
+    p[i] = as_u32(__hsub2(as_bf2(lop_and_or(w >> (4 * i), mask, 0x43004300u)), as_bf2(0x43084308u)));
 }
 
 // The codes of an 8-bit word (two's complement bytes) as two bf16 pairs: 128 +
 // the low seven bits, minus 128 or 256 by the sign bit (0x4380 is 256); exact.
-__device__ __forceinline__ void codes8(uint32_t w, uint32_t* p) {
+__device__ __forceinline__ void codes8(uint32_t w, uint32_t mask, uint32_t* p) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t u = w >> (8 * i);
-    p[i] = as_u32(__hsub2(as_bf2(lop_and_or(u, 0x007F007Fu, 0x43004300u)), as_bf2(lop_and_or(u, 0x00800080u, 0x43004300u))));
+    p[i] = as_u32(__hsub2(as_bf2(lop_and_or(u, mask, 0x43004300u)), as_bf2(lop_and_or(u, mask + 0x00010001u, 0x43004300u))));
   }
 }
 
@@ -343,10 +356,10 @@ __global__ void __launch_bounds__(256) read_kernel(ReadParams p, long long items
       const uint32_t s2 = j == 0 ? sc.x : sc.y;
       const __nv_bfloat162 d = as_bf2(__byte_perm(s2, s2, grp == 0 ? 0x1010 : 0x3232));
       if (BITS == 4) {
-        codes4(a[j][0], o);
+        codes4(a[j][0], code_mask<4>(), o);
       } else {
-        codes8(a[j][0], o);
-        codes8(a[j][1], o + 2);
+        codes8(a[j][0], code_mask<8>(), o);
+        codes8(a[j][1], code_mask<8>(), o + 2);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[i] = as_u32(__hmul2(as_bf2(o[i]), d));
