@@ -38,9 +38,9 @@ struct AttnParams {
   float scale_log2;
   uint32_t mask;     // code_mask<BITS>()
   int row_blocks;    // blocks of 8 * NT rows per (sequence, kv head)
-  int parts, per;    // splits along the keys: units per part
-  float* part_o;     // [(b, h, row block)][part][8 NT][64], when parts > 1
-  float* part_ml;    // [...][8 NT][2]
+  int split;         // 0: one CTA per (block of rows, kv head); 1: all units dealt out to the CTAs evenly
+  float* part_o;     // split: [CTA][2][8 NT][64]
+  float* part_ml;    //        [CTA][2][8 NT][2]
 };
 
 // What a block of rows [r0, r0 + n) of one sequence sees: units (pages) [0, sink) and
@@ -50,7 +50,6 @@ struct Span {
   int lo, hi;     // positions of the first and last row's token
   int sink, first, count;
   int open, shut, sink_open;  // units that every row sees whole: [open, shut) and [0, sink_open)
-  int per;  // units of a part: the plan's, or more where the sequence is longer than the plan was made for
   __device__ __forceinline__ int unit(int u) const { return u < sink ? u : first + u - sink; }
   __device__ __forceinline__ int pos(int i, int causal) const { return causal ? len - ql + i : len - 1; }
 };
@@ -68,7 +67,6 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int r0, int 
   s.lo = s.pos(i0, p.causal);
   s.hi = s.pos(i1, p.causal);
   s.sink = s.first = s.count = s.open = s.shut = s.sink_open = 0;
-  s.per = p.per;
   if (i0 > i1 || s.hi < 0) return s;
   s.shut = max(0, s.lo + 1) / kUnit;
   if (p.window > 0) {
@@ -78,7 +76,6 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int r0, int 
     s.sink = min((p.sinks + kUnit - 1) / kUnit, s.first);
   }
   s.count = s.sink + s.hi / kUnit - s.first + 1;
-  s.per = max(p.per, (s.count + p.parts - 1) / p.parts);
   return s;
 }
 
@@ -226,28 +223,116 @@ constexpr int attend_smem() {
   return rings > join ? rings : join;
 }
 
-// One CTA per (part, kv head, row block, sequence): its warps take the part's
-// units in turn, each with its own running maximum, sum and output, which are
-// joined in shared memory at the end.  A warp copies half pages into its own ring
-// ahead of its computation (cp.async; no warp waits for another).
+// Groups are blocks of rows of a sequence (b, rb), items a group's kv heads; the
+// units of all items in order, group by group and head by head, make one line.
+// With `split` the line is cut into n shares that differ by one unit at most, so
+// lengths however uneven leave no CTA waiting for another; n is the grid, or
+// fewer when that would leave CTAs less than a unit per warp.  (Fewer than 2^31
+// units: the host checks.)
+struct Deal {
+  int n, share, extra;  // the first `extra` shares have one unit more
+  __device__ __forceinline__ int begin(int c) const { return c * share + min(c, extra); }
+  __device__ __forceinline__ int owner(int unit) const {
+    const int long_ones = extra * (share + 1);
+    return unit < long_ones ? unit / (share + 1) : extra + (unit - long_ones) / share;
+  }
+};
+__device__ __forceinline__ Deal deal_of(int total, int ctas) {
+  Deal d;
+  d.n = max(1, min(ctas, (total + kWarps - 1) / kWarps));
+  d.share = total / d.n;
+  d.extra = total - d.share * d.n;
+  return d;
+}
+
+// The sum of all threads' values; *before: of the threads below.
+template <int THREADS>
+__device__ __forceinline__ int block_scan(int v, int* before, int* shared) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int run = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, d);
+    if (lane >= d) run += up;
+  }
+  if (lane == 31) shared[warp] = run;
+  __syncthreads();
+  int base = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) base += shared[w];
+    total += shared[w];
+  }
+  *before = base + run - v;
+  return total;
+}
+
+// A CTA's warps take the units of an item (or of its share of one) in turn, each
+// with its own running maximum, sum and output, which are joined in shared memory
+// at the item's end.  A warp copies pages into its own ring ahead of its
+// computation (cp.async; no warp waits for another).
 template <int BITS, int NT>
 __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   pdl_prologue();
-  constexpr int R = 8 * NT;
+  constexpr int R = 8 * NT, kThreads = kWarps * 32;
   using Rg = Ring<BITS>;
-  extern __shared__ __align__(128) uint8_t smem[];  // the rings; after the loop the warps' results
+  extern __shared__ __align__(128) uint8_t smem[];  // the rings; after an item's loop the warps' results
+  __shared__ int s_scan[kWarps];
+  __shared__ int s_group, s_left;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  int x = blockIdx.x;  // kv head, part, row block, sequence
-  const int h = x % p.c.kv_heads;
-  x /= p.c.kv_heads;
-  const int part = x % p.parts;
-  x /= p.parts;
-  const int rb = x % p.row_blocks, b = x / p.row_blocks;
-  const int rows = p.Lq * p.G, r0 = rb * R;
-  const Span sp = span_of(p, b, r0, R);
-  const int u0 = part * sp.per, u1 = min(sp.count, u0 + sp.per);
-  if (part > 0 && u0 >= sp.count) return;  // part 0 writes the rows that see nothing
+  const int rows = p.Lq * p.G, heads = p.c.kv_heads, groups = p.c.batch * p.row_blocks;
 
+  // where this CTA starts, and how many units it takes
+  int group, h, u0, left;
+  if (p.split) {
+    const int chunk = (groups + kThreads - 1) / kThreads;
+    const int ga = min(groups, (int)threadIdx.x * chunk), gb = min(groups, ga + chunk);
+    int mine = 0, before;
+    for (int i = ga; i < gb; ++i) mine += span_of(p, i / p.row_blocks, i % p.row_blocks * R, R).count;
+    const Deal d = deal_of(heads * block_scan<kThreads>(mine, &before, s_scan), gridDim.x);
+    const int f0 = d.begin(blockIdx.x);
+    left = (int)blockIdx.x < d.n ? d.begin(blockIdx.x + 1) - f0 : 0;
+    if (left > 0 && f0 >= before * heads && f0 < (before + mine) * heads) {  // one thread's groups hold it
+      int at = f0 - before * heads;
+      int i = ga;
+      for (;; ++i) {
+        const int here = heads * span_of(p, i / p.row_blocks, i % p.row_blocks * R, R).count;
+        if (at < here) break;
+        at -= here;
+      }
+      s_group = i;
+      s_left = at;
+    }
+    // rows that see nothing belong to no unit
+    for (int i = blockIdx.x; i < groups; i += gridDim.x) {
+      const int b = i / p.row_blocks, r0 = i % p.row_blocks * R;
+      if (span_of(p, b, r0, R).count > 0) continue;
+      for (int x = threadIdx.x; x < heads * R * 8; x += kThreads) {
+        const int hh = x / (R * 8), row = r0 + (x >> 3) % R, qi = row / p.G;
+        if (row < rows)
+          *reinterpret_cast<uint4*>(p.o + (long long)b * p.o_batch + (long long)qi * p.o_row +
+                                    (long long)(hh * p.G + row - qi * p.G) * HD + (x & 7) * 8) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (left == 0) return;
+    __syncthreads();
+    group = s_group;
+    const int count = span_of(p, group / p.row_blocks, group % p.row_blocks * R, R).count;
+    h = s_left / count;
+    u0 = s_left - h * count;
+  } else {
+    group = blockIdx.x / heads;
+    h = blockIdx.x - group * heads;
+    u0 = 0;
+    left = 0x7FFFFFFF;
+  }
+
+  for (int segment = 0; left > 0; ++segment) {
+  const int b = group / p.row_blocks, r0 = group % p.row_blocks * R;
+  const Span sp = span_of(p, b, r0, R);
+  const int u1 = min(sp.count - u0, left) + u0;
+
+  // the units' pages
   const int* table = p.c.table + (long long)b * p.c.table_ld;
   auto page_of = [&](int u) { return u < u1 ? table[sp.unit(u)] : 0; };  // slots lie inside the table (span_of)
   auto block = [&](int u, int page) -> const uint8_t* {
@@ -256,7 +341,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
       vla_record_error(VLA_DERR_KV_RANGE);
       return nullptr;
     }
-    return p.c.pool + ((long long)page * p.c.kv_heads + h) * Block<BITS>::kBytes;
+    return p.c.pool + ((long long)page * heads + h) * Block<BITS>::kBytes;
   };
   const int steps = u0 + warp < u1 ? Rg::kSteps * ((u1 - u0 - warp + kWarps - 1) / kWarps) : 0;
   const uint32_t ring = smem_u32(smem) + warp * Rg::kWarpBytes;
@@ -509,8 +594,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
     }
   }
   __syncthreads();
-  const bool whole = sp.count <= sp.per;  // the only part of these rows
-  const long long slot = (((long long)b * p.row_blocks + rb) * p.c.kv_heads + h) * p.parts + part;
+  const bool whole = u0 == 0 && u1 == sp.count;
+  const long long slot = 2ll * blockIdx.x + (segment > 0 ? 1 : 0);  // a CTA has at most two items in part: its first and last
   for (int y = threadIdx.x; y < R * 8; y += kWarps * 32) {
     const int r = y >> 3, d8 = (y & 7) * 8, row = r0 + r;
     if (row >= rows) continue;
@@ -541,37 +626,60 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
       if (d8 == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * R + r) * 2) = make_float2(top, sum);
     }
   }
+  if (!p.split) return;
+  left -= u1 - u0;
+  if (left > 0) {  // the next item that has units
+    u0 = 0;
+    if (++h == heads) {
+      h = 0;
+      do ++group;
+      while (span_of(p, group / p.row_blocks, group % p.row_blocks * R, R).count == 0);
+    }
+    __syncthreads();  // the results' memory is the next item's ring
+  }
+  }
 }
 
-// Joins the parts of a row, in an order that their number alone sets: one CTA
-// per row of a kv head, each warp a share of the parts, two dims per lane.
+// Joins the parts of a row, in the order of their CTAs: one CTA per row of a kv
+// head, each warp a share of the parts, two dims per lane.
 constexpr int kJoinWarps = 8;
 template <int NT>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p, int ctas) {
   pdl_prologue();
-  constexpr int R = 8 * NT;
+  constexpr int R = 8 * NT, kThreads = kJoinWarps * 32;
   __shared__ float sO[kJoinWarps][HD];
   __shared__ float sL[kJoinWarps];
-  const int rows = p.Lq * p.G;
-  const long long hb = blockIdx.x / rows;  // kv head, sequence
-  const int row = (int)(blockIdx.x - hb * rows);
-  const int h = (int)(hb % p.c.kv_heads), b = (int)(hb / p.c.kv_heads);
+  __shared__ int s_scan[kJoinWarps], s_before[kJoinWarps];
+  const int rows = p.Lq * p.G, heads = p.c.kv_heads, groups = p.c.batch * p.row_blocks;
+  const int hb = blockIdx.x / rows, row = blockIdx.x - hb * rows;
+  const int h = hb % heads, b = hb / heads;
   const int rb = row / R, r = row - rb * R, i = row / p.G, head = h * p.G + row - i * p.G;
+  const int group = b * p.row_blocks + rb;
   const Span sp = span_of(p, b, rb * R, R);
-  if (sp.count <= sp.per) return;  // written whole
-  const int n = (sp.count + sp.per - 1) / sp.per;
+  if (sp.count == 0) return;
+  // the item's units in the line of all
+  int all = 0, below = 0, unused;
+  for (int y = threadIdx.x; y < groups; y += kThreads) {
+    const int n = span_of(p, y / p.row_blocks, y % p.row_blocks * R, R).count;
+    all += n;
+    below += y < group ? n : 0;
+  }
+  const Deal d = deal_of(heads * block_scan<kThreads>(all, &unused, s_scan), ctas);
+  const int start = heads * block_scan<kThreads>(below, &unused, s_before) + h * sp.count;
+  const int c0 = d.owner(start), n = d.owner(start + sp.count - 1) - c0 + 1;
+  if (n == 1) return;  // written whole
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long slot = (((long long)b * p.row_blocks + rb) * p.c.kv_heads + h) * p.parts;
-  const float* ml = p.part_ml + (slot * R + r) * 2;
-  const float* po = p.part_o + (slot * R + r) * HD + 2 * lane;
+  // a part is its CTA's first item, but the first part may be its CTA's last
+  const int late = start > d.begin(c0) ? 1 : 0;
+  auto slot = [&](int y) { return (2ll * (c0 + y) + (y == 0 ? late : 0)) * R + r; };
   float top = -INFINITY;
-  for (int y = lane; y < n; y += 32) top = fmaxf(top, ml[(long long)y * (2 * R)]);
+  for (int y = lane; y < n; y += 32) top = fmaxf(top, p.part_ml[slot(y) * 2]);
   top = warp_max(top);
   float sum = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll 4
   for (int y = warp; y < n; y += kJoinWarps) {
-    const float2 v = *reinterpret_cast<const float2*>(po + (long long)y * (R * HD));
-    const float2 w = *reinterpret_cast<const float2*>(ml + (long long)y * (2 * R));
+    const float2 v = *reinterpret_cast<const float2*>(p.part_o + slot(y) * HD + 2 * lane);
+    const float2 w = *reinterpret_cast<const float2*>(p.part_ml + slot(y) * 2);
     const float f = w.x == -INFINITY ? 0.f : ex2((w.x - top) * p.scale_log2);
     sum += w.x == -INFINITY ? w.y : f * w.y;
     a0 += f * v.x;

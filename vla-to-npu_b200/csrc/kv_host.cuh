@@ -91,17 +91,41 @@ static int read(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, 
   return launch_status("kv_read");
 }
 
-// Row tile and key splits of a call; both depend on its sizes alone.
+// Row tile, split and workspace of a call; they depend on its sizes alone.
 struct Plan {
-  int nt, row_blocks, parts, per;
+  int nt, row_blocks, split;
   size_t workspace;
 };
+
+template <int BITS, int NT>
+static int resident_ctas() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>& n = cached[dev & 63];
+  if (n.load(std::memory_order_relaxed) == 0) {
+    constexpr int smem = attend_smem<BITS, NT>();
+    int per = 0;
+    if (cudaFuncSetAttribute(attend_kernel<BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attend_kernel<BITS, NT>, kWarps * 32, smem) != cudaSuccess ||
+        per < 1) {
+      cudaGetLastError();  // no device: sizes are still answered
+      return 4 * device_info().num_sms;
+    }
+    n.store(per * device_info().num_sms, std::memory_order_relaxed);
+  }
+  return n.load(std::memory_order_relaxed);
+}
+static int resident_ctas(int bits, int nt) {
+  if (bits == 4) return nt == 1 ? resident_ctas<4, 1>() : nt == 2 ? resident_ctas<4, 2>() : resident_ctas<4, 4>();
+  return nt == 1 ? resident_ctas<8, 1>() : nt == 2 ? resident_ctas<8, 2>() : resident_ctas<8, 4>();
+}
 
 static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a, Plan* out) {
   const long long rows = (long long)a->Lq * (a->Hq / c->kv_heads);
   VLA_CHECK_ARG(rows < (1ll << 30), "kv_attention: too many query rows");
   out->nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  out->row_blocks = (int)((rows + 8 * out->nt - 1) / (8 * out->nt));
+  const long long blocks = (rows + 8 * out->nt - 1) / (8 * out->nt);
   const long long room = (long long)c->max_pages * kPage;
   long long keys = a->max_len > 0 && a->max_len < room ? a->max_len : room;
   if (a->window > 0) {
@@ -109,19 +133,12 @@ static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a,
     const long long seen = (long long)a->window + a->sinks + (8 * out->nt - 1) / (a->Hq / c->kv_heads) + 3 * kUnit;
     if (seen < keys) keys = seen;
   }
-  const long long units = (keys + kUnit - 1) / kUnit;
-  const long long base = (long long)c->batch * c->kv_heads * out->row_blocks;
-  static const int per_sm = []() { const char* e = getenv("KV_PER_SM"); return e ? atoi(e) : 12; }();
-  static const int min_units = []() { const char* e = getenv("KV_MIN_UNITS"); return e ? atoi(e) : 8; }();
-  const long long want = ((long long)per_sm * device_info().num_sms + base - 1) / base;
-  const long long most = (units + min_units - 1) / min_units;
-  long long parts = want < most ? want : most;
-  if (parts < 1) parts = 1;
-  out->per = (int)((units + parts - 1) / parts);
-  if (out->per < 1) out->per = 1;
-  out->parts = (int)parts;
-  VLA_CHECK_ARG(base * parts < (1ll << 31), "kv_attention: too many work items");
-  out->workspace = parts > 1 ? (size_t)base * parts * 8 * out->nt * (HD + 2) * sizeof(float) : 0;
+  VLA_CHECK_ARG(c->batch * blocks * c->kv_heads <= ((1ll << 31) - 1) / (c->max_pages > 0 ? c->max_pages : 1) && c->batch * rows * c->kv_heads < (1ll << 31),
+                "kv_attention: too many work items");
+  out->row_blocks = (int)blocks;
+  out->split = keys > 8 * kUnit;
+  out->workspace =
+      out->split ? (size_t)resident_ctas(c->bits, out->nt) * 2 * 8 * out->nt * (HD + 2) * sizeof(float) : 0;
   return VLA_OK;
 }
 
@@ -136,15 +153,13 @@ static int check_attention(const vla_kv_cache* c, const vla_kv_attention_args* a
 }
 
 template <int BITS, int NT>
-static int launch_attend(const AttnParams& p, const Plan& pl, cudaStream_t st) {
+static void launch_attend(const AttnParams& p, cudaStream_t st) {
   constexpr int smem = attend_smem<BITS, NT>();
-  VLA_CUDA_TRY(cudaFuncSetAttribute(attend_kernel<BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const long long base = (long long)p.c.batch * p.c.kv_heads * pl.row_blocks;
-  launch_k(attend_kernel<BITS, NT>, dim3((unsigned)(base * pl.parts)), dim3(kWarps * 32), smem, st, p);
-  if (pl.parts > 1)
-    launch_k(join_kernel<NT>, dim3((unsigned)((long long)p.c.batch * p.c.kv_heads * p.Lq * p.G)), dim3(kJoinWarps * 32),
-             0, st, p);
-  return VLA_OK;
+  const int ctas = resident_ctas<BITS, NT>();
+  const int items = p.c.batch * p.row_blocks * p.c.kv_heads;
+  launch_k(attend_kernel<BITS, NT>, dim3(p.split ? ctas : items), dim3(kWarps * 32), smem, st, p);
+  if (p.split)
+    launch_k(join_kernel<NT>, dim3(p.c.batch * p.c.kv_heads * p.Lq * p.G), dim3(kJoinWarps * 32), 0, st, p, ctas);
 }
 
 static size_t attention_workspace(const vla_kv_cache* c, const vla_kv_attention_args* a) {
@@ -188,27 +203,23 @@ static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cuda
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.mask = c->bits == 4 ? code_mask<4>() : code_mask<8>();
   p.row_blocks = pl.row_blocks;
-  p.parts = pl.parts;
-  p.per = pl.per;
+  p.split = pl.split;
   p.part_o = (float*)a->workspace;
-  if (pl.parts > 1)
-    p.part_ml = p.part_o + (size_t)c->batch * c->kv_heads * pl.row_blocks * pl.parts * 8 * pl.nt * HD;
-  int rc;
+  if (pl.split) p.part_ml = p.part_o + pl.workspace / sizeof(float) / (HD + 2) * HD;
   prof_begin(st);
   if (c->bits == 4) {
-    if (pl.nt == 1) rc = launch_attend<4, 1>(p, pl, st);
-    else if (pl.nt == 2) rc = launch_attend<4, 2>(p, pl, st);
-    else rc = launch_attend<4, 4>(p, pl, st);
+    if (pl.nt == 1) launch_attend<4, 1>(p, st);
+    else if (pl.nt == 2) launch_attend<4, 2>(p, st);
+    else launch_attend<4, 4>(p, st);
   } else {
-    if (pl.nt == 1) rc = launch_attend<8, 1>(p, pl, st);
-    else if (pl.nt == 2) rc = launch_attend<8, 2>(p, pl, st);
-    else rc = launch_attend<8, 4>(p, pl, st);
+    if (pl.nt == 1) launch_attend<8, 1>(p, st);
+    else if (pl.nt == 2) launch_attend<8, 2>(p, st);
+    else launch_attend<8, 4>(p, st);
   }
   // the lengths are on the device: the profile counts whole caches (or windows)
-  const double keys = (double)pl.per * pl.parts * kUnit;
+  const double keys = a->window > 0 && a->window < room ? (double)a->window + a->sinks : (double)room;
   prof_end(st, VLA_KIND_ATTENTION, 4.0 * c->batch * a->Hq * (double)a->Lq * keys * HD,
            c->batch * (keys * c->kv_heads * block_bytes(c->bits) / kPage + 4.0 * a->Lq * a->Hq * HD));
-  VLA_TRY(rc);
   return launch_status("kv_attention");
 }
 
