@@ -41,6 +41,7 @@ struct AttnParams {
   int split;         // 0: one CTA per (block of rows, kv head); 1: all units dealt out to the CTAs evenly
   float* part_o;     // split: [CTA][2][8 NT][64]
   float* part_ml;    //        [CTA][2][8 NT][2]
+  int4* cut;         //        [CTA]: the item that starts in this CTA and goes on in others
 };
 
 // What a block of rows [r0, r0 + n) of one sequence sees: units (pages) [0, sink) and
@@ -227,7 +228,7 @@ constexpr int attend_smem() {
 // units of all items in order, group by group and head by head, make one line.
 // With `split` the line is cut into n shares that differ by one unit at most, so
 // lengths however uneven leave no CTA waiting for another; n is the grid, or
-// fewer when that would leave CTAs less than a unit per warp.  (Fewer than 2^31
+// fewer when that would leave CTAs less than `least` units.  (Fewer than 2^31
 // units: the host checks.)
 struct Deal {
   int n, share, extra;  // the first `extra` shares have one unit more
@@ -237,9 +238,9 @@ struct Deal {
     return unit < long_ones ? unit / (share + 1) : extra + (unit - long_ones) / share;
   }
 };
-__device__ __forceinline__ Deal deal_of(int total, int ctas) {
+__device__ __forceinline__ Deal deal_of(int total, int ctas, int least) {
   Deal d;
-  d.n = max(1, min(ctas, (total + kWarps - 1) / kWarps));
+  d.n = max(1, min(ctas, (total + least - 1) / least));
   d.share = total / d.n;
   d.extra = total - d.share * d.n;
   return d;
@@ -267,6 +268,17 @@ __device__ __forceinline__ int block_scan(int v, int* before, int* shared) {
   return total;
 }
 
+// What CTA c's share ends with, for join_kernel: group, kv head, slot of the first
+// part, number of parts (0: its last item ends with the share or started before).
+__device__ __forceinline__ void record_cut(const AttnParams& p, const Deal& d, int group, int h, int u0, int u1,
+                                           int units, int segment) {
+  const int c = blockIdx.x;
+  if (u1 < units)
+    p.cut[c] = u0 == 0 ? make_int4(group, h, 2 * c + (segment > 0 ? 1 : 0),
+                                   d.owner(d.begin(c + 1) - u1 + units - 1) - c + 1)
+                       : make_int4(0, 0, 0, 0);
+}
+
 // A CTA's warps take the units of an item (or of its share of one) in turn, each
 // with its own running maximum, sum and output, which are joined in shared memory
 // at the item's end.  A warp copies pages into its own ring ahead of its
@@ -284,12 +296,13 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
 
   // where this CTA starts, and how many units it takes
   int group, h, u0, left;
+  Deal d{};
   if (p.split) {
     const int chunk = (groups + kThreads - 1) / kThreads;
     const int ga = min(groups, (int)threadIdx.x * chunk), gb = min(groups, ga + chunk);
     int mine = 0, before;
     for (int i = ga; i < gb; ++i) mine += span_of(p, i / p.row_blocks, i % p.row_blocks * R, R).count;
-    const Deal d = deal_of(heads * block_scan<kThreads>(mine, &before, s_scan), gridDim.x);
+    d = deal_of(heads * block_scan<kThreads>(mine, &before, s_scan), gridDim.x, kWarps);
     const int f0 = d.begin(blockIdx.x);
     left = (int)blockIdx.x < d.n ? d.begin(blockIdx.x + 1) - f0 : 0;
     if (left > 0 && f0 >= before * heads && f0 < (before + mine) * heads) {  // one thread's groups hold it
@@ -314,6 +327,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
                                     (long long)(hh * p.G + row - qi * p.G) * HD + (x & 7) * 8) = make_uint4(0, 0, 0, 0);
       }
     }
+    if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (left == 0) return;
     __syncthreads();
     group = s_group;
@@ -627,6 +641,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
     }
   }
   if (!p.split) return;
+  if (threadIdx.x == 0) record_cut(p, d, group, h, u0, u1, sp.count, segment);
   left -= u1 - u0;
   if (left > 0) {  // the next item that has units
     u0 = 0;
@@ -640,68 +655,57 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   }
 }
 
-// Joins the parts of a row, in the order of their CTAs: one CTA per row of a kv
-// head, each warp a share of the parts, two dims per lane.
+// Joins the parts of cut items, in the order of their CTAs: kWarpsPerRow warps per
+// row share the parts, two dims per lane.  blockIdx: (slice of the rows, CTA).
 constexpr int kJoinWarps = 8;
-template <int NT>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p, int ctas) {
+template <int R, int WPR>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p, float to_log2) {
   pdl_prologue();
-  constexpr int R = 8 * NT, kThreads = kJoinWarps * 32;
   __shared__ float sO[kJoinWarps][HD];
   __shared__ float sL[kJoinWarps];
-  __shared__ int s_scan[kJoinWarps], s_before[kJoinWarps];
-  const int rows = p.Lq * p.G, heads = p.c.kv_heads, groups = p.c.batch * p.row_blocks;
-  const int hb = blockIdx.x / rows, row = blockIdx.x - hb * rows;
-  const int h = hb % heads, b = hb / heads;
-  const int rb = row / R, r = row - rb * R, i = row / p.G, head = h * p.G + row - i * p.G;
-  const int group = b * p.row_blocks + rb;
-  const Span sp = span_of(p, b, rb * R, R);
-  if (sp.count == 0) return;
-  // the item's units in the line of all
-  int all = 0, below = 0, unused;
-  for (int y = threadIdx.x; y < groups; y += kThreads) {
-    const int n = span_of(p, y / p.row_blocks, y % p.row_blocks * R, R).count;
-    all += n;
-    below += y < group ? n : 0;
-  }
-  const Deal d = deal_of(heads * block_scan<kThreads>(all, &unused, s_scan), ctas);
-  const int start = heads * block_scan<kThreads>(below, &unused, s_before) + h * sp.count;
-  const int c0 = d.owner(start), n = d.owner(start + sp.count - 1) - c0 + 1;
-  if (n == 1) return;  // written whole
+  const int4 cut = p.cut[blockIdx.y];
+  const int n = cut.w;
+  if (n == 0) return;
+  const int b = cut.x / p.row_blocks, h = cut.y, r0 = cut.x % p.row_blocks * R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x * (kJoinWarps / WPR) + warp / WPR, row = r0 + r;
+  const bool there = r < R && row < p.Lq * p.G;
   // a part is its CTA's first item, but the first part may be its CTA's last
-  const int late = start > d.begin(c0) ? 1 : 0;
-  auto slot = [&](int y) { return (2ll * (c0 + y) + (y == 0 ? late : 0)) * R + r; };
-  float top = -INFINITY;
-  for (int y = lane; y < n; y += 32) top = fmaxf(top, p.part_ml[slot(y) * 2]);
-  top = warp_max(top);
+  auto slot = [&](int y) { return (long long)(y == 0 ? cut.z : 2 * ((int)blockIdx.y + y)) * R + r; };
   float sum = 0.f, a0 = 0.f, a1 = 0.f;
+  if (there) {
+    float top = -INFINITY;
+    for (int y = lane; y < n; y += 32) top = fmaxf(top, p.part_ml[slot(y) * 2]);
+    top = warp_max(top);
 #pragma unroll 4
-  for (int y = warp; y < n; y += kJoinWarps) {
-    const float2 v = *reinterpret_cast<const float2*>(p.part_o + slot(y) * HD + 2 * lane);
-    const float2 w = *reinterpret_cast<const float2*>(p.part_ml + slot(y) * 2);
-    const float f = w.x == -INFINITY ? 0.f : ex2((w.x - top) * p.scale_log2);
-    sum += w.x == -INFINITY ? w.y : f * w.y;
-    a0 += f * v.x;
-    a1 += f * v.y;
-  }
-  sO[warp][2 * lane] = a0;
-  sO[warp][2 * lane + 1] = a1;
-  if (lane == 0) sL[warp] = sum;
-  __syncthreads();
-  if (warp == 0) {
-    sum = a0 = a1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      sum += sL[w];
-      a0 += sO[w][2 * lane];
-      a1 += sO[w][2 * lane + 1];
+    for (int y = warp % WPR; y < n; y += WPR) {
+      const float2 v = *reinterpret_cast<const float2*>(p.part_o + slot(y) * HD + 2 * lane);
+      const float2 w = *reinterpret_cast<const float2*>(p.part_ml + slot(y) * 2);
+      const float f = w.x == -INFINITY ? 0.f : ex2((w.x - top) * to_log2);
+      sum += w.x == -INFINITY ? w.y : f * w.y;
+      a0 += f * v.x;
+      a1 += f * v.y;
     }
-    const bool empty = i >= sp.ql || sum == 0.f;
-    const float inv = empty ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint32_t*>(p.o + (long long)b * p.o_batch + (long long)i * p.o_row + (long long)head * HD +
-                                 2 * lane) = empty ? 0u : pack_bf16x2(a0 * inv, a1 * inv);
   }
+  if (WPR > 1) {
+    sO[warp][2 * lane] = a0;
+    sO[warp][2 * lane + 1] = a1;
+    if (lane == 0) sL[warp] = sum;
+    __syncthreads();
+    if (warp % WPR != 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) {
+      sum += sL[warp + w];
+      a0 += sO[warp + w][2 * lane];
+      a1 += sO[warp + w][2 * lane + 1];
+    }
+  }
+  if (!there) return;
+  const int i = row / p.G, head = h * p.G + row - i * p.G;
+  const bool empty = (p.q_len != nullptr && i >= p.q_len[b]) || sum == 0.f;
+  const float inv = empty ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint32_t*>(p.o + (long long)b * p.o_batch + (long long)i * p.o_row + (long long)head * HD +
+                               2 * lane) = empty ? 0u : pack_bf16x2(a0 * inv, a1 * inv);
 }
 
 }  // namespace kv

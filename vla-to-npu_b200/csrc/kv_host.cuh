@@ -5,6 +5,7 @@
 
 #include "host_common.cuh"
 #include "kv_attention.cuh"
+#include "kv_attention_tc.cuh"
 #include "kvcache.cuh"
 
 namespace vla {
@@ -93,7 +94,8 @@ static int read(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, 
 
 // Row tile, split and workspace of a call; they depend on its sizes alone.
 struct Plan {
-  int nt, row_blocks, split;
+  int nt;          // 8-row tiles of the mma.sync kernel, 0: the tcgen05 kernel
+  int block, row_blocks, split;  // rows of a block, blocks per (sequence, kv head)
   size_t workspace;
 };
 
@@ -124,21 +126,23 @@ static int resident_ctas(int bits, int nt) {
 static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a, Plan* out) {
   const long long rows = (long long)a->Lq * (a->Hq / c->kv_heads);
   VLA_CHECK_ARG(rows < (1ll << 30), "kv_attention: too many query rows");
-  out->nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  const long long blocks = (rows + 8 * out->nt - 1) / (8 * out->nt);
+  out->nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
+  const int block = out->nt > 0 ? 8 * out->nt : tc::kRows;
+  const long long blocks = (rows + block - 1) / block;
   const long long room = (long long)c->max_pages * kPage;
   long long keys = a->max_len > 0 && a->max_len < room ? a->max_len : room;
   if (a->window > 0) {
     // the window of a block's rows and the first tokens, in whole pages
-    const long long seen = (long long)a->window + a->sinks + (8 * out->nt - 1) / (a->Hq / c->kv_heads) + 3 * kUnit;
+    const long long seen = (long long)a->window + a->sinks + (block - 1) / (a->Hq / c->kv_heads) + 3 * kUnit;
     if (seen < keys) keys = seen;
   }
   VLA_CHECK_ARG(c->batch * blocks * c->kv_heads <= ((1ll << 31) - 1) / (c->max_pages > 0 ? c->max_pages : 1) && c->batch * rows * c->kv_heads < (1ll << 31),
                 "kv_attention: too many work items");
+  out->block = block;
   out->row_blocks = (int)blocks;
-  out->split = keys > 8 * kUnit;
-  out->workspace =
-      out->split ? (size_t)resident_ctas(c->bits, out->nt) * 2 * 8 * out->nt * (HD + 2) * sizeof(float) : 0;
+  out->split = out->nt == 0 || keys > 8 * kUnit;
+  const size_t ctas = out->nt == 0 ? device_info().num_sms : out->split ? resident_ctas(c->bits, out->nt) : 0;
+  out->workspace = ctas * (2 * block * (HD + 2) * sizeof(float) + sizeof(int4));
   return VLA_OK;
 }
 
@@ -158,8 +162,33 @@ static void launch_attend(const AttnParams& p, cudaStream_t st) {
   const int ctas = resident_ctas<BITS, NT>();
   const int items = p.c.batch * p.row_blocks * p.c.kv_heads;
   launch_k(attend_kernel<BITS, NT>, dim3(p.split ? ctas : items), dim3(kWarps * 32), smem, st, p);
-  if (p.split)
-    launch_k(join_kernel<NT>, dim3(p.c.batch * p.c.kv_heads * p.Lq * p.G), dim3(kJoinWarps * 32), 0, st, p, ctas);
+  if (p.split) {  // a CTA per row that is there
+    const int slices = p.row_blocks > 1 ? 8 * NT : p.Lq * p.G;
+    launch_k(join_kernel<8 * NT, kJoinWarps>, dim3(slices, ctas), dim3(kJoinWarps * 32), 0, st, p, p.scale_log2);
+  }
+}
+
+template <int BITS>
+static int launch_tc(const AttnParams& p, cudaStream_t st) {
+  constexpr int smem = tc::smem_bytes<BITS>();
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    VLA_CUDA_TRY(cudaFuncSetAttribute(tc::attend_kernel<BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaFuncAttributes fa{};
+    VLA_CUDA_TRY(cudaFuncGetAttributes(&fa, tc::attend_kernel<BITS>));
+    // setmaxnreg hands out exactly the launch's registers: only sound at the count it was sized for
+    if (fa.numRegs != tc::kLaunchRegs)
+      return set_error(VLA_E_CUDA, "kv_attention: built with %d registers per thread, sized for %d", fa.numRegs,
+                       tc::kLaunchRegs);
+    ready.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+  }
+  const int ctas = device_info().num_sms;
+  launch_k(tc::attend_kernel<BITS>, dim3(ctas), dim3(tc::kThreads), smem, st, p);
+  const int slices = ((p.row_blocks > 1 ? tc::kRows : p.Lq * p.G) + kJoinWarps - 1) / kJoinWarps;
+  launch_k(join_kernel<tc::kRows, 1>, dim3(slices, ctas), dim3(kJoinWarps * 32), 0, st, p, 1.f);
+  return VLA_OK;
 }
 
 static size_t attention_workspace(const vla_kv_cache* c, const vla_kv_attention_args* a) {
@@ -205,9 +234,15 @@ static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cuda
   p.row_blocks = pl.row_blocks;
   p.split = pl.split;
   p.part_o = (float*)a->workspace;
-  if (pl.split) p.part_ml = p.part_o + pl.workspace / sizeof(float) / (HD + 2) * HD;
+  if (pl.split) {
+    const size_t rows = pl.workspace / (2 * pl.block * (HD + 2) * sizeof(float) + sizeof(int4)) * 2 * pl.block;
+    p.part_ml = p.part_o + rows * HD;
+    p.cut = reinterpret_cast<int4*>(p.part_ml + rows * 2);
+  }
   prof_begin(st);
-  if (c->bits == 4) {
+  if (pl.nt == 0) {
+    VLA_TRY(c->bits == 4 ? launch_tc<4>(p, st) : launch_tc<8>(p, st));
+  } else if (c->bits == 4) {
     if (pl.nt == 1) launch_attend<4, 1>(p, st);
     else if (pl.nt == 2) launch_attend<4, 2>(p, st);
     else launch_attend<4, 4>(p, st);
