@@ -129,7 +129,7 @@ __device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, 
                                         int lane) {
   constexpr int C = Raw<BITS>::kCodes;
   const int g = lane >> 2, t = lane & 3;
-#pragma unroll
+#pragma unroll 1
   for (int tile = 0; tile < 2; ++tile) {
     const uint32_t sc = raw + 2 * C + tile * 128;
     // keys: tokens a and a + 2, 8 dims of either group
@@ -544,19 +544,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           const int ua = 2 * (wk.u0 + j), ka = sp.unit(ua), kb = sp.unit(ua + 1);  // pages
           bool plain = ((ka >= sp.open && ka < sp.shut) || ka < sp.sink_open) &&
                        ((kb >= sp.open && kb < sp.shut) || kb < sp.sink_open);
-          uint32_t absent = 0;  // per 32 keys
+          uint32_t vis[4] = {0u, 0u, 0u, 0u};  // keys that the row sees, set where not all are
           {
             const uint32_t f = smem_u32(&sm.flags[t % kFlags]);
             const uint4 n0 = lds16(f), n1 = lds16(f + 16), ab = lds16(f + 32);
-            absent = ab.x | ab.y << 1 | ab.z << 2 | ab.w << 3;
-            plain = plain && absent == 0u;
-            if ((n0.x | n0.y | n0.z | n0.w | n1.x | n1.y | n1.z | n1.w) != 0u) {
-              const uint32_t v0 = seen32(ka * kUnit, pos, p.window, p.sinks);
-              const uint32_t v1 = seen32(ka * kUnit + 32, pos, p.window, p.sinks);
-              const uint32_t v2 = seen32(kb * kUnit, pos, p.window, p.sinks);
-              const uint32_t v3 = seen32(kb * kUnit + 32, pos, p.window, p.sinks);
-              if (((n0.x & v0) | (n0.y & v1) | (n0.z & v2) | (n0.w & v3)) != 0u) nan |= 1u;
-              if (((n1.x & v0) | (n1.y & v1) | (n1.z & v2) | (n1.w & v3)) != 0u) nan |= 2u;
+            const uint32_t flagged = n0.x | n0.y | n0.z | n0.w | n1.x | n1.y | n1.z | n1.w;
+            plain = plain && (ab.x | ab.z) == 0u;
+            if (!plain || flagged != 0u) {
+              vis[0] = ab.x != 0u ? 0u : seen32(ka * kUnit, pos, p.window, p.sinks);
+              vis[1] = ab.x != 0u ? 0u : seen32(ka * kUnit + 32, pos, p.window, p.sinks);
+              vis[2] = ab.z != 0u ? 0u : seen32(kb * kUnit, pos, p.window, p.sinks);
+              vis[3] = ab.z != 0u ? 0u : seen32(kb * kUnit + 32, pos, p.window, p.sinks);
+              if (((n0.x & vis[0]) | (n0.y & vis[1]) | (n0.z & vis[2]) | (n0.w & vis[3])) != 0u) nan |= 1u;
+              if (((n1.x & vis[0]) | (n1.y & vis[1]) | (n1.z & vis[2]) | (n1.w & vis[3])) != 0u) nan |= 2u;
             }
           }
           // Half of the row at a time, so that it fits the registers: the first half is
@@ -565,12 +565,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           auto load = [&](int half) {
             tmem_ld64(s_adr + half * kUnit, sr);
             if (!plain) {
-              const int k0 = (half == 0 ? ka : kb) * kUnit;
-              const int hi = ((absent >> (2 * half)) & 1u) ? -1 : pos - k0;
-              const int lo = p.window > 0 ? pos - p.window - k0 : -1, first = p.window > 0 ? p.sinks - k0 : 0;
+              const uint32_t v0 = half == 0 ? vis[0] : vis[2], v1 = half == 0 ? vis[1] : vis[3];
 #pragma unroll
-              for (int c = 0; c < kUnit; ++c)
-                if (c > hi || (c <= lo && c >= first)) sr[c] = -INFINITY;
+              for (int c = 0; c < 32; ++c) {
+                sr[c] = (v0 >> c) & 1u ? sr[c] : -INFINITY;
+                sr[32 + c] = (v1 >> c) & 1u ? sr[32 + c] : -INFINITY;
+              }
             }
           };
           auto top = [&]() {
@@ -625,15 +625,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           if (!idle) {
             const float mbase = m == -INFINITY ? 0.f : m;
             float rs[4] = {0.f, 0.f, 0.f, 0.f};
-            // (the polynomial does not go below 2^-126, and a key that is not seen has to
-            // give 0: units with such keys take every exponential from the MUFU)
-            auto exps = [&](int half, auto poly) {
+#pragma unroll 1
+            for (int half = 1; half >= 0; --half) {
+              if (half == 0) {
+                load(0);
+                tc_fence_before();
+                mbar_arrive(&sm.s_free[g]);
+              }
               uint32_t pk[kUnit / 2];
 #pragma unroll
               for (int c = 0; c < kUnit; c += 2) {
                 float x0, x1, e0, e1;
                 attn_tc::fma2(sr[c], sr[c + 1], p.scale_log2, -mbase, x0, x1);
-                if (decltype(poly)::value && ((c >> 1) & 7) < 2) {
+                if (((c >> 1) & 7) < 2) {
                   attn_tc::ex2_poly2(x0, x1, e0, e1);
                 } else {
                   e0 = ex2(x0);
@@ -642,22 +646,23 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
                 attn_tc::add2(rs[c & 2], rs[(c & 2) + 1], e0, e1);
                 pk[c >> 1] = pack_bf16x2(e0, e1);
               }
+              if (!plain) {  // the polynomial ends at 2^-126: a key that is not seen gives 0
+                const uint32_t v0 = half == 0 ? vis[0] : vis[2], v1 = half == 0 ? vis[1] : vis[3];
+#pragma unroll
+                for (int c = 0; c < kUnit; c += 16) {  // the pairs that took it
+#pragma unroll
+                  for (int e = c; e < c + 4; e += 2) {
+                    const uint32_t two = (e < 32 ? v0 : v1) >> (e & 31);
+                    pk[e >> 1] &= ((two & 1u) ? 0x0000FFFFu : 0u) | ((two & 2u) ? 0xFFFF0000u : 0u);
+                  }
+                }
+              }
               attn_tc::tmem_st32(p_adr + half * (kUnit / 2), pk);
-            };
-            if (plain)
-              exps(1, std::true_type());
-            else
-              exps(1, std::false_type());
-            load(0);
-            tc_fence_before();
-            mbar_arrive(&sm.s_free[g]);
-            if (plain)
-              exps(0, std::true_type());
-            else
-              exps(0, std::false_type());
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.mufu_tok[g ^ 1][q]);
-            l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+            const float sum = (rs[0] + rs[1]) + (rs[2] + rs[3]);
+            l += m == -INFINITY && sum == sum ? 0.f : sum;  // no key seen yet: the polynomial's 2^-126 do not count
           } else {
             mbar_arrive(&sm.s_free[g]);
             if (lane == 0) mbar_arrive(&sm.mufu_tok[g ^ 1][q]);
