@@ -73,7 +73,6 @@ struct Smem {
   uint64_t k_full[kRing], k_empty[kRing];
   uint64_t v_full[kRing], v_empty[kRing];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
-  uint64_t mufu_tok[2][4];
   int scan[kThreads / 32];
   int group, left;
   uint32_t tmem_base;
@@ -228,6 +227,36 @@ __device__ __forceinline__ void finish_row(const AttnParams& p, uint32_t o_adr, 
   if (!whole && row < rows) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m, l);
 }
 
+__device__ __forceinline__ void tmem_start32(uint32_t a, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(a));
+}
+// waits for the loads in flight; the registers pass through it, so no use moves above
+__device__ __forceinline__ void tmem_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+        "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+        "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+        "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :: "memory");
+}
+__device__ __forceinline__ void tmem_put16(uint32_t a, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(a),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 template <int BITS>
 __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -244,7 +273,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
       mbar_init(&sm.s_free[i], 128);
       mbar_init(&sm.p_full[i], 128);
       mbar_init(&sm.pv_done[i], 1);
-      for (int q = 0; q < 4; ++q) mbar_init(&sm.mufu_tok[i][q], 1);
     }
     for (int s = 0; s < kRing; ++s) {
       mbar_init(&sm.k_full[s], 4);
@@ -559,44 +587,57 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
               if (((n1.x & vis[0]) | (n1.y & vis[1]) | (n1.z & vis[2]) | (n1.w & vis[3])) != 0u) nan |= 2u;
             }
           }
-          // Half of the row at a time, so that it fits the registers: the first half is
-          // read for its maximum only and again for its exponentials.
-          float sr[kUnit];
-          auto load = [&](int half) {
-            tmem_ld64(s_adr + half * kUnit, sr);
+          // The row goes by in quarters, the next one on its way from TMEM.  Exponentials
+          // are taken against the maximum so far while the unit's own is still being
+          // found; where that outgrows it by more than 2^8 (the first unit, then rarely)
+          // the quarters are gone through again.
+          uint32_t sa[2][32];
+          auto mask = [&](uint32_t* r, int qt) {
             if (!plain) {
-              const uint32_t v0 = half == 0 ? vis[0] : vis[2], v1 = half == 0 ? vis[1] : vis[3];
+              const uint32_t v = qt == 0 ? vis[0] : qt == 1 ? vis[1] : qt == 2 ? vis[2] : vis[3];
 #pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                sr[c] = (v0 >> c) & 1u ? sr[c] : -INFINITY;
-                sr[32 + c] = (v1 >> c) & 1u ? sr[32 + c] : -INFINITY;
+              for (int c = 0; c < 32; ++c) r[c] = (v >> c) & 1u ? r[c] : 0xFF800000u;
+            }
+          };
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto top = [&](const uint32_t* r) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
+            }
+          };
+          float rs[4] = {0.f, 0.f, 0.f, 0.f};
+          auto exps = [&](const uint32_t* r, int qt) {
+            const float mbase = m == -INFINITY ? 0.f : m;
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float x0, x1, e0, e1;
+              attn_tc::fma2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]), p.scale_log2, -mbase, x0, x1);
+              if (((c >> 1) & 7) < 2) {
+                attn_tc::ex2_poly2(x0, x1, e0, e1);
+              } else {
+                e0 = ex2(x0);
+                e1 = ex2(x1);
+              }
+              attn_tc::add2(rs[c & 2], rs[(c & 2) + 1], e0, e1);
+              pk[c >> 1] = pack_bf16x2(e0, e1);
+            }
+            if (!plain) {  // the polynomial ends at 2^-126: a key that is not seen gives 0
+              const uint32_t v = qt == 0 ? vis[0] : qt == 1 ? vis[1] : qt == 2 ? vis[2] : vis[3];
+#pragma unroll
+              for (int c = 0; c < 32; c += 16) {  // the pairs that took it
+#pragma unroll
+                for (int e = c; e < c + 4; e += 2) {
+                  const uint32_t two = v >> e;
+                  pk[e >> 1] &= ((two & 1u) ? 0x0000FFFFu : 0u) | ((two & 2u) ? 0xFFFF0000u : 0u);
+                }
               }
             }
+            tmem_put16(p_adr + qt * 16, pk);
           };
-          auto top = [&]() {
-            float mx4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx4[e] = max3(sr[e], sr[4 + e], sr[8 + e]);
-#pragma unroll
-            for (int c = 12; c < kUnit; c += 8) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], sr[c + e], sr[min(c + 4 + e, kUnit - 1)]);
-            }
-            return max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3]));
-          };
-          float mx = -INFINITY;
-          if (!idle) {
-            load(0);
-            mx = top();
-            load(1);
-            mx = fmaxf(mx, top()) * p.scale_log2;
-          }
-          const bool grow = mx > m + kRescaleLog2;
-          const float alpha = grow ? ex2(m - mx) : 1.f;
-          if (grow) {
-            m = mx;
-            l *= alpha;
-          }
+          if (!idle) tmem_start32(s_adr, sa[0]);
           if (t > 0) {
             // P_g and O_g were last used by P.V of unit t - 1
             ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
@@ -604,68 +645,88 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             if (!ok) break;
             tc_fence_after();
           }
-          if (j == 0 && pending) {
-            finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
-            pending = false;
-          }
-          if (j > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-              float o[16];
-              uint32_t u[16];
-              tmem_ld16(o_adr + c, o);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
-              attn_tc::tmem_st16(o_adr + c, u);
-            }
-          }
-          ok = mbar_wait_bounded(&sm.mufu_tok[g][q], g == 0 ? (((uint32_t)t & 1u) ^ 1u) : ((uint32_t)t & 1u), abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
           if (!idle) {
-            const float mbase = m == -INFINITY ? 0.f : m;
-            float rs[4] = {0.f, 0.f, 0.f, 0.f};
+            bool again = j == 0;
+            if (!again) {
 #pragma unroll 1
-            for (int half = 1; half >= 0; --half) {
-              if (half == 0) {
-                load(0);
-                tc_fence_before();
-                mbar_arrive(&sm.s_free[g]);
-              }
-              uint32_t pk[kUnit / 2];
-#pragma unroll
-              for (int c = 0; c < kUnit; c += 2) {
-                float x0, x1, e0, e1;
-                attn_tc::fma2(sr[c], sr[c + 1], p.scale_log2, -mbase, x0, x1);
-                if (((c >> 1) & 7) < 2) {
-                  attn_tc::ex2_poly2(x0, x1, e0, e1);
-                } else {
-                  e0 = ex2(x0);
-                  e1 = ex2(x1);
-                }
-                attn_tc::add2(rs[c & 2], rs[(c & 2) + 1], e0, e1);
-                pk[c >> 1] = pack_bf16x2(e0, e1);
-              }
-              if (!plain) {  // the polynomial ends at 2^-126: a key that is not seen gives 0
-                const uint32_t v0 = half == 0 ? vis[0] : vis[2], v1 = half == 0 ? vis[1] : vis[3];
-#pragma unroll
-                for (int c = 0; c < kUnit; c += 16) {  // the pairs that took it
-#pragma unroll
-                  for (int e = c; e < c + 4; e += 2) {
-                    const uint32_t two = (e < 32 ? v0 : v1) >> (e & 31);
-                    pk[e >> 1] &= ((two & 1u) ? 0x0000FFFFu : 0u) | ((two & 2u) ? 0xFFFF0000u : 0u);
+              for (int qt = 0; qt < 4; qt += 2) {
+                tmem_wait32(sa[0]);
+                tmem_start32(s_adr + 32 * qt + 32, sa[1]);
+                mask(sa[0], qt);
+                top(sa[0]);
+                exps(sa[0], qt);
+                tmem_wait32(sa[1]);
+                if (qt == 0) tmem_start32(s_adr + 64, sa[0]);
+                mask(sa[1], qt + 1);
+                top(sa[1]);
+                if (qt == 2) {
+                  const float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+                  again = __any_sync(0xffffffffu, mx > m + kRescaleLog2);
+                  if (!again) {
+                    tc_fence_before();
+                    mbar_arrive(&sm.s_free[g]);
                   }
                 }
+                exps(sa[1], qt + 1);
               }
-              attn_tc::tmem_st32(p_adr + half * (kUnit / 2), pk);
+            } else {
+              tmem_wait32(sa[0]);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.mufu_tok[g ^ 1][q]);
+            if (j == 0 && pending) {
+              finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
+              pending = false;
+            }
+            if (again) {
+#pragma unroll 1
+              for (int qt = 0; qt < 4; ++qt) {
+                tmem_start32(s_adr + 32 * qt, sa[0]);
+                tmem_wait32(sa[0]);
+                mask(sa[0], qt);
+                top(sa[0]);
+              }
+              const float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+              float alpha = 1.f;
+              if (mx > m + kRescaleLog2) {
+                alpha = ex2(m - mx);
+                m = mx;
+                l *= alpha;
+              }
+              if (j > 0) {
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 16) {
+                  float o[16];
+                  uint32_t u[16];
+                  tmem_ld16(o_adr + c, o);
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
+                  attn_tc::tmem_st16(o_adr + c, u);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) rs[e] = 0.f;
+              tmem_put_wait();
+#pragma unroll 1
+              for (int qt = 0; qt < 4; ++qt) {
+                tmem_start32(s_adr + 32 * qt, sa[0]);
+                tmem_wait32(sa[0]);
+                if (qt == 3) {
+                  tc_fence_before();
+                  mbar_arrive(&sm.s_free[g]);
+                }
+                mask(sa[0], qt);
+                exps(sa[0], qt);
+              }
+            }
+            tmem_put_wait();
             const float sum = (rs[0] + rs[1]) + (rs[2] + rs[3]);
             l += m == -INFINITY && sum == sum ? 0.f : sum;  // no key seen yet: the polynomial's 2^-126 do not count
           } else {
+            if (j == 0 && pending) {
+              finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
+              pending = false;
+            }
+            tc_fence_before();
             mbar_arrive(&sm.s_free[g]);
-            if (lane == 0) mbar_arrive(&sm.mufu_tok[g ^ 1][q]);
           }
           tc_fence_before();
           mbar_arrive(&sm.p_full[g]);
