@@ -158,6 +158,8 @@ CASES = [
     (150, 3, 1, [260, 150], [150, 130], True, 100, 1),
     (1, 3, 1, [500], None, True, 10, 490),
     (4, 6, 2, [500], None, False, 1, 1),
+    (33, 8, 8, [1 + 37 * i % 128 for i in range(96)], None, True, 0, 0),  # many short sequences per CTA
+    (40, 4, 4, [37 * i % 300 for i in range(70)], None, False, 0, 0),
 ]
 
 

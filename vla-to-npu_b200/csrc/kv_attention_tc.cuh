@@ -62,6 +62,20 @@ struct Flags {
   uint32_t absent[4];  // per 32 keys: not there
 };
 
+// A CTA's share of an item, as warp 0 hands it to the other roles.
+struct Segment {
+  Span sp;
+  int b, h, r0;        // sequence, kv head, first row
+  int u0, n;           // units [u0, u0 + n)
+  int whole;           // ... are all of the item's
+  int more;            // another segment follows
+  long long slot;      // of its part in the workspace, in rows
+};
+// Entries: warp 0 writes segment i + 8's when S of segment i + 5 is complete, by which
+// time every role is past segment i.  (It is written before the wait for a free query
+// buffer: the copies ahead of the conversion need it while that buffer is in use.)
+constexpr int kSegments = 8;
+
 template <int BITS>
 struct Smem {
   uint8_t q[2][2][TILE_BYTES];  // [buffer][tile]
@@ -69,6 +83,8 @@ struct Smem {
   uint8_t v[kRing][TILE_BYTES];
   uint8_t raw[4][Raw<BITS>::kStages][Raw<BITS>::kBytes];  // [warp]
   Flags flags[kFlags];
+  Segment seg[kSegments];
+  uint64_t seg_full[kSegments];
   uint64_t q_full[2], q_empty[2];
   uint64_t k_full[kRing], k_empty[kRing];
   uint64_t v_full[kRing], v_empty[kRing];
@@ -83,23 +99,6 @@ struct Smem {
 __device__ __forceinline__ int units_of(const AttnParams& p, int group) {
   return (span_of(p, group / p.row_blocks, group % p.row_blocks * kRows, kRows).count + 1) / 2;
 }
-
-// The shares of an item that a CTA walks through.
-struct Walk {
-  int group, h, u0, left;
-  // `units`: of the current item; steps to the next share, false at the end
-  __device__ __forceinline__ bool next(const AttnParams& p, int units) {
-    left -= min(units - u0, left);
-    if (left <= 0) return false;
-    u0 = 0;
-    if (++h == p.c.kv_heads) {
-      h = 0;
-      do ++group;
-      while (units_of(p, group) == 0);
-    }
-    return true;
-  }
-};
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -124,8 +123,8 @@ __device__ __forceinline__ uint32_t seen32(int key0, int pos, int window, int si
 
 // 32 keys' codes to rows [r0, r0 + 32) of a K and a V tile.
 template <int BITS>
-__device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, int r0, int live, uint32_t mask,
-                                        int lane) {
+__device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, int r0, int live, bool clean,
+                                        uint32_t mask, int lane) {
   constexpr int C = Raw<BITS>::kCodes;
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll 1
@@ -172,10 +171,12 @@ __device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int rr = r0 + tile * 16 + 4 * q + r;
-      uint32_t s = 4 * q + r + tile * 16 < live ? vs[r] : 0u;
-      uint32_t d0 = lo2(s), d1 = hi2(s);
-      if ((d0 & 0x7F80u) == 0x7F80u) d0 = 0u;  // NaN: flagged
-      if ((d1 & 0x7F80u) == 0x7F80u) d1 = 0u;
+      uint32_t d0 = lo2(vs[r]), d1 = hi2(vs[r]);
+      if (!clean) {  // past the end, or NaN (flagged)
+        const bool past = 4 * q + r + tile * 16 >= live;
+        if (past || (d0 & 0x7F80u) == 0x7F80u) d0 = 0u;
+        if (past || (d1 & 0x7F80u) == 0x7F80u) d1 = 0u;
+      }
       uint32_t c[4];
       if (BITS == 4) {
         codes4(r == 0 ? w0.x : r == 1 ? w0.y : r == 2 ? w0.z : w0.w, mask, c);
@@ -197,7 +198,7 @@ __device__ __forceinline__ void finish_row(const AttnParams& p, uint32_t o_adr, 
   const int rows = p.Lq * p.G, i = row / p.G, head = h * p.G + row - i * p.G;
   const bool empty = i >= ql || l == 0.f;
   const float inv = !whole ? 1.f : empty ? 0.f : 1.f / l;
-#pragma unroll
+#pragma unroll 1
   for (int half = 0; half < 2; ++half) {
     float o[HD / 2];
     tmem_ld32(o_adr + (uint32_t)half * (HD / 2), o);  // warp-collective: every lane loads
@@ -274,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
       mbar_init(&sm.p_full[i], 128);
       mbar_init(&sm.pv_done[i], 1);
     }
+    for (int s = 0; s < kSegments; ++s) mbar_init(&sm.seg_full[s], 1);
     for (int s = 0; s < kRing; ++s) {
       mbar_init(&sm.k_full[s], 4);
       mbar_init(&sm.k_empty[s], 2);
@@ -297,12 +299,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
     const int chunk = (groups + kThreads - 1) / kThreads;
     const int ga = min(groups, (int)threadIdx.x * chunk), gb = min(groups, ga + chunk);
     int mine = 0, before;
+#pragma unroll 1
     for (int i = ga; i < gb; ++i) mine += units_of(p, i);
     d = deal_of(heads * block_scan<kThreads>(mine, &before, sm.scan), gridDim.x, 1);
     const int f0 = d.begin(blockIdx.x);
     left = (int)blockIdx.x < d.n ? d.begin(blockIdx.x + 1) - f0 : 0;
     if (left > 0 && f0 >= before * heads && f0 < (before + mine) * heads) {
       int at = f0 - before * heads, i = ga;
+#pragma unroll 1
       for (;; ++i) {
         const int here = heads * units_of(p, i);
         if (at < here) break;
@@ -313,9 +317,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
     }
     if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
     // rows that see nothing belong to no unit
+#pragma unroll 1
     for (int i = blockIdx.x; i < groups; i += gridDim.x) {
       const int b = i / p.row_blocks, r0 = i % p.row_blocks * kRows;
       if (units_of(p, i) > 0) continue;
+#pragma unroll 1
       for (int x = threadIdx.x; x < heads * kRows * 8; x += kThreads) {
         const int hh = x / (kRows * 8), row = r0 + (x >> 3) % kRows, qi = row / p.G;
         if (row < rows)
@@ -326,24 +332,42 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
     __syncthreads();
   }
   if (left > 0) {
-    Walk wk;
-    {
-      const int units = units_of(p, sm.group);
-      wk = Walk{sm.group, sm.left / units, sm.left % units, left};
-    }
     bool ok = true;
+    int it = 0;  // segments
+    auto segment = [&](int i) -> const Segment& {
+      ok = mbar_wait_bounded(&sm.seg_full[i % kSegments], (i / kSegments) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      return sm.seg[i % kSegments];
+    };
     if (warp < 4) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
       if (warp == 0) {
-        // ---------------- queries ----------------
-        int it = 0;
-        bool more = true;
-        while (more && ok) {
-          const int b = wk.group / p.row_blocks, r0 = wk.group % p.row_blocks * kRows, qb = it & 1;
+        // ---------------- segments and queries ----------------
+        int group = sm.group, units = units_of(p, group), h = sm.left / units, u0 = sm.left - h * units;
+#pragma unroll 1
+        for (; ok && left > 0; ++it) {
+          const int b = group / p.row_blocks, r0 = (group - b * p.row_blocks) * kRows, qb = it & 1;
+          const int n = min(units - u0, left);
+          left -= n;
+          if (lane == 0) {
+            Segment& sg = sm.seg[it % kSegments];
+            sg.sp = span_of(p, b, r0, kRows);
+            sg.b = b;
+            sg.h = h;
+            sg.r0 = r0;
+            sg.u0 = u0;
+            sg.n = n;
+            sg.whole = n == units;
+            sg.more = left > 0;
+            sg.slot = (2ll * blockIdx.x + (it > 0 ? 1 : 0)) * kRows;
+            mbar_arrive(&sm.seg_full[it % kSegments]);
+            record_cut(p, d, group, h, u0, u0 + n, units, it);
+          }
+          __syncwarp();
           ok = mbar_wait_bounded(&sm.q_empty[qb], ((it >> 1) & 1) ^ 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const bf16* src = p.q + (long long)b * p.q_batch + (long long)wk.h * p.G * HD + (lane & 7) * 8;
+          const bf16* src = p.q + (long long)b * p.q_batch + (long long)h * p.G * HD + (lane & 7) * 8;
           const uint32_t dst = smem_u32(sm.q[qb][0]);
           int r = lane >> 3, i = (r0 + r) / p.G, hh = r0 + r - i * p.G;
           const int di = 4 / p.G, dh = 4 - di * p.G;
@@ -363,26 +387,34 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             }
           }
           copy_commit();
+          // the next item that has units
+          u0 = 0;
+          if (++h == heads && left > 0) {
+            h = 0;
+#pragma unroll 1
+            do units = units_of(p, ++group);
+            while (units == 0);
+          }
           copy_wait<0>();
           fence_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.q_full[qb]);
-          const int units = units_of(p, wk.group);
-          if (lane == 0) record_cut(p, d, wk.group, wk.h, wk.u0, wk.u0 + min(units - wk.u0, wk.left), units, it);
-          ++it;
-          more = wk.next(p, units);
         }
       } else if (warp < 3) {
         // ---------------- S issuers ----------------
         const int g = warp - 1;
         constexpr uint32_t idesc_s = make_idesc_bf16(BQ, kKeys);
         const uint32_t s_tmem = tmem + S_COL0 + (uint32_t)g * kKeys;
-        int t = 0, it = 0;
-        bool more = true;
-        while (more && ok) {
-          const int units = units_of(p, wk.group), n = min(units - wk.u0, wk.left), qb = it & 1;
+        int t = 0;
+#pragma unroll 1
+        for (bool more = true; more && ok; ++it) {
+          const Segment& sg = segment(it);
+          if (!ok) break;
+          const int n = sg.n, qb = it & 1;
+          more = sg.more;
           ok = mbar_wait_bounded(&sm.q_full[qb], (it >> 1) & 1, abort_flag);
           const uint64_t qdesc = make_sw128_desc(smem_u32(sm.q[qb][g]));
+#pragma unroll 1
           for (int j = 0; ok && j < n; ++j, ++t) {
             const int sk = t % kRing;
             ok = mbar_wait_bounded(&sm.k_full[sk], (t / kRing) & 1, abort_flag);
@@ -401,18 +433,21 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           if (!ok) break;
           if (elect_one()) tc_commit(&sm.q_empty[qb]);
           __syncwarp();
-          ++it;
-          more = wk.next(p, units);
         }
       } else {
         // ---------------- P.V issuer ----------------
         constexpr uint32_t idesc_pv = make_idesc_bf16(BQ, HD) | (1u << 16);  // B (V) is MN-major
         int t = 0;
-        bool more = true;
-        while (more && ok) {
-          const int units = units_of(p, wk.group), n = min(units - wk.u0, wk.left);
+#pragma unroll 1
+        for (bool more = true; more && ok; ++it) {
+          const Segment& sg = segment(it);
+          if (!ok) break;
+          const int n = sg.n;
+          more = sg.more;
+#pragma unroll 1
           for (int j = 0; ok && j < n; ++j, ++t) {
             const int sv = t % kRing;
+#pragma unroll 1
             for (int g = 0; g < 2; ++g) {
               ok = mbar_wait_bounded(&sm.p_full[g], (uint32_t)t & 1u, abort_flag);
               if (ok) ok = mbar_wait_bounded(&sm.v_full[sv], (t / kRing) & 1, abort_flag);
@@ -433,7 +468,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
               __syncwarp();
             }
           }
-          more = wk.next(p, units);
         }
       }
     } else if (warp < 8) {
@@ -442,21 +476,39 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
       using Rw = Raw<BITS>;
       const int w = warp - 4;  // keys [32 w, 32 w + 32) of a unit: half (w & 1) of page w >> 1
       const uint32_t raw = smem_u32(sm.raw[w]);
-      // copies run kStages - 1 units ahead with a walk of their own
-      Walk cw = wk;
-      Span csp = span_of(p, cw.group / p.row_blocks, cw.group % p.row_blocks * kRows, kRows);
-      int cu = cw.u0, cend = cw.u0 + min((csp.count + 1) / 2 - cw.u0, cw.left), ct = 0;
+      // copies run kStages - 1 units ahead, with a segment count of their own
+      int ci = 0, cu = 0, cn = 0, ct = 0, cpage = 0, cb = 0, ch = 0;
+      int csink = 0, cfirst = 0, ccount = 0;
       bool cmore = true;
       uint32_t there = 0;  // bit (stage): the page exists
+      auto page_ahead = [&]() {  // the next copy's page number
+        const int u = 2 * cu + (w >> 1);
+        if (u < ccount) cpage = p.c.table[(long long)cb * p.c.table_ld + (u < csink ? u : cfirst + u - csink)];
+      };
+      auto copy_segment = [&]() {
+        const Segment& sg = segment(ci);
+        ++ci;
+        if (!ok) return;
+        cu = sg.u0;
+        cn = sg.n;
+        cb = sg.b;
+        ch = sg.h;
+        csink = sg.sp.sink;
+        cfirst = sg.sp.first;
+        ccount = sg.sp.count;
+        cmore = sg.more;
+        page_ahead();
+      };
+      copy_segment();
       auto copy_next = [&]() {
-        if (cmore) {
+        if (cn == 0 && cmore) copy_segment();
+        if (cn > 0 && ok) {
           const int st = ct % Rw::kStages, u = 2 * cu + (w >> 1);
           bool have = false;
-          if (u < csp.count) {
-            const int page = p.c.table[(long long)(cw.group / p.row_blocks) * p.c.table_ld + csp.unit(u)];
-            have = page >= 0 && page < p.c.pages;
+          if (u < ccount) {
+            have = cpage >= 0 && cpage < p.c.pages;
             if (have) {
-              const uint8_t* blk = p.c.pool + ((long long)page * heads + cw.h) * Block<BITS>::kBytes;
+              const uint8_t* blk = p.c.pool + ((long long)cpage * heads + ch) * Block<BITS>::kBytes;
               const uint32_t dst = raw + st * Rw::kBytes + lane * 16;
               const uint8_t* src = blk + (w & 1) * Rw::kCodes + lane * 16;
 #pragma unroll
@@ -472,24 +524,24 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           }
           there = have ? there | (1u << st) : there & ~(1u << st);
           ++ct;
-          if (++cu == cend) {
-            cmore = cw.next(p, (csp.count + 1) / 2);
-            if (cmore) {
-              csp = span_of(p, cw.group / p.row_blocks, cw.group % p.row_blocks * kRows, kRows);
-              cu = cw.u0;
-              cend = cu + min((csp.count + 1) / 2 - cu, cw.left);
-            }
-          }
+          ++cu;
+          if (--cn > 0)
+            page_ahead();
+          else if (cmore && __all_sync(0xffffffffu, mbar_test(&sm.seg_full[ci % kSegments], (ci / kSegments) & 1)))
+            copy_segment();
         }
         copy_commit();
       };
 #pragma unroll
       for (int i = 0; i < Rw::kStages - 1; ++i) copy_next();
       int t = 0;
-      bool more = true;
-      while (more && ok) {
-        const Span sp = span_of(p, wk.group / p.row_blocks, wk.group % p.row_blocks * kRows, kRows);
-        const int units = (sp.count + 1) / 2, n = min(units - wk.u0, wk.left);
+#pragma unroll 1
+      for (bool more = ok; more && ok; ++it) {
+        const Segment& sg = segment(it);
+        if (!ok) break;
+        const int n = sg.n, u0 = sg.u0, len = sg.sp.len, sink = sg.sp.sink, first = sg.sp.first;
+        more = sg.more;
+#pragma unroll 1
         for (int j = 0; ok && j < n; ++j, ++t) {
           const int st = t % Rw::kStages, sr = t % kRing;
           const bool have = (there >> st) & 1u;  // before copy_next changes another stage's bit
@@ -501,12 +553,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const uint32_t kt = smem_u32(sm.k[sr]), vt = smem_u32(sm.v[sr]), from = raw + st * Rw::kBytes;
-          const int u = 2 * (wk.u0 + j) + (w >> 1);
+          const int u = 2 * (u0 + j) + (w >> 1), page = u < sink ? u : first + u - sink;
           int live = 0;  // of the 32 keys, those inside the sequence
           uint32_t n0 = 0u, n1 = 0u;
           if (have) {
-            live = min(32, sp.len - (sp.unit(u) * kUnit + (w & 1) * 32));
-            convert<BITS>(from, kt, vt, w * 32, live, p.mask, lane);
+            live = min(32, len - (page * kUnit + (w & 1) * 32));
             // key `lane`: tile lane / 16, token 4 q + b + 2 c at (2 q + b) * 16 + c * 8
             const int tk = lane & 15;
             uint32_t s;
@@ -516,6 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
                                ((tk >> 1) & 1) * 8 + 4));
             n0 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F80u) == 0x7F80u);
             n1 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F800000u) == 0x7F800000u);
+            convert<BITS>(from, kt, vt, w * 32, live, live == 32 && (n0 | n1) == 0u, p.mask, lane);
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -536,8 +588,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             mbar_arrive(&sm.v_full[sr]);
           }
         }
-        if (!ok) break;
-        more = wk.next(p, units);
       }
       copy_wait<0>();
     } else {
@@ -549,27 +599,39 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
       const uint32_t p_adr = tmem + lane_base + P_COL0 + (uint32_t)g * (kKeys / 2);
       const uint32_t o_adr = tmem + lane_base + O_COL0 + (uint32_t)g * HD;
       int t = 0;
-      // the previous share's O_g is read out before this share's first P_g is released
-      bool pending = false, pend_whole = false, more = true;
-      int pend_b = 0, pend_h = 0, pend_ql = 0, pend_row = 0, segment = 0;
+      // a segment's O_g is read out before the next one's first P_g is released
+      bool pending = false, pend_whole = false;
+      int pend_b = 0, pend_h = 0, pend_ql = 0, pend_row = 0;
       long long pend_slot = 0;
       float pend_m = 0.f, pend_l = 0.f;
       uint32_t pend_nan = 0;
-      while (more && ok) {
-        const int b = wk.group / p.row_blocks, r0 = wk.group % p.row_blocks * kRows;
-        const Span sp = span_of(p, b, r0, kRows);
-        const int units = (sp.count + 1) / 2, n = min(units - wk.u0, wk.left);
+#pragma unroll 1
+      for (bool more = true; ok; ++it) {
+        if (pending) {
+          ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
+        }
+        if (!more) break;
+        const Segment& sg = segment(it);
+        if (!ok) break;
+        more = sg.more;
+        const Span sp = sg.sp;
+        const int u0 = sg.u0, n = sg.n, r0 = sg.r0;
         const int row = r0 + g * BQ + q * 32 + lane, i = row / p.G;
         const int pos = row < rows && i < sp.ql ? sp.pos(i, p.causal) : -1;
         const bool idle = r0 + g * BQ + q * 32 >= rows;  // no row in this warp
         float m = -INFINITY, l = 0.f;
         uint32_t nan = 0;
+#pragma unroll 1
         for (int j = 0; j < n; ++j, ++t) {
           ok = mbar_wait_bounded(&sm.s_full[g], (uint32_t)t & 1u, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          const int ua = 2 * (wk.u0 + j), ka = sp.unit(ua), kb = sp.unit(ua + 1);  // pages
+          const int ua = 2 * (u0 + j), ka = sp.unit(ua), kb = sp.unit(ua + 1);  // pages
           bool plain = ((ka >= sp.open && ka < sp.shut) || ka < sp.sink_open) &&
                        ((kb >= sp.open && kb < sp.shut) || kb < sp.sink_open);
           uint32_t vis[4] = {0u, 0u, 0u, 0u};  // keys that the row sees, set where not all are
@@ -672,10 +734,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             } else {
               tmem_wait32(sa[0]);
             }
-            if (j == 0 && pending) {
-              finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
-              pending = false;
-            }
             if (again) {
 #pragma unroll 1
               for (int qt = 0; qt < 4; ++qt) {
@@ -721,10 +779,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             const float sum = (rs[0] + rs[1]) + (rs[2] + rs[3]);
             l += m == -INFINITY && sum == sum ? 0.f : sum;  // no key seen yet: the polynomial's 2^-126 do not count
           } else {
-            if (j == 0 && pending) {
-              finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
-              pending = false;
-            }
             tc_fence_before();
             mbar_arrive(&sm.s_free[g]);
           }
@@ -733,19 +787,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
         }
         if (!ok) break;
         pending = true;
-        pend_whole = n == units;
-        pend_b = b, pend_h = wk.h, pend_ql = sp.ql, pend_row = row, pend_m = m, pend_l = l, pend_nan = nan;
-        pend_slot = (2ll * blockIdx.x + (segment > 0 ? 1 : 0)) * kRows + (row - r0);
-        ++segment;
-        more = wk.next(p, units);
-      }
-      if (ok && pending) {
-        ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) {
-          tc_fence_after();
-          finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
-        }
+        pend_whole = sg.whole != 0;
+        pend_b = sg.b, pend_h = sg.h, pend_ql = sp.ql, pend_row = row, pend_m = m, pend_l = l, pend_nan = nan;
+        pend_slot = sg.slot + (row - r0);
       }
     }
     if (!ok && lane == 0) {
