@@ -37,7 +37,7 @@ struct AttnParams {
   int causal, window, sinks;
   float scale_log2;
   uint32_t mask;     // code_mask<BITS>()
-  int row_blocks;    // blocks of 8 * NT rows per (sequence, kv head)
+  int block, row_blocks;  // rows of a block, blocks per (sequence, kv head)
   int split;         // 0: one CTA per (block of rows, kv head); 1: all units dealt out to the CTAs evenly
   float* part_o;     // split: [CTA][2][8 NT][64]
   float* part_ml;    //        [CTA][2][8 NT][2]
@@ -666,10 +666,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(AttnParams p, flo
   const int4 cut = p.cut[blockIdx.y];
   const int n = cut.w;
   if (n == 0) return;
-  const int b = cut.x / p.row_blocks, h = cut.y, r0 = cut.x % p.row_blocks * R;
+  const int b = cut.x / p.row_blocks, h = cut.y, r0 = cut.x % p.row_blocks * p.block;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.x * (kJoinWarps / WPR) + warp / WPR, row = r0 + r;
-  const bool there = r < R && row < p.Lq * p.G;
+  const bool there = r < p.block && row < p.Lq * p.G;
   // a part is its CTA's first item, but the first part may be its CTA's last
   auto slot = [&](int y) { return (long long)(y == 0 ? cut.z : 2 * ((int)blockIdx.y + y)) * R + r; };
   float sum = 0.f, a0 = 0.f, a1 = 0.f;

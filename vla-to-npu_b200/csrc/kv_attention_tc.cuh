@@ -9,7 +9,7 @@
 // dealt out evenly to the persistent CTAs (kv_attention.cuh), so causal masks,
 // windows and uneven lengths leave no SM waiting; an item cut by a CTA's border
 // leaves fp32 sums that join_kernel adds.  Warp roles:
-//   warp 0       queries (cp.async into 128-byte-swizzled tiles, double-buffered)
+//   warp 0       the CTA's segments (shares of items), for the other roles
 //   warps 1, 2   S issuers, one per group: S_g = Q_g K^T (128 x 128 into TMEM)
 //   warp 3       P.V issuer: O_g += P_g V (P from TMEM, V as the MN-major operand)
 //   warps 4..7   codes to bf16: each takes 32 keys of the unit, copies their codes
@@ -18,9 +18,8 @@
 //                rings.  Against a bf16 cache this is what the kernel adds: about
 //                320 instructions per thread and unit beside the softmax's 2000
 //                issue slots.
-//   warps 8..15  softmax: one thread per row, as in attention_tc.cuh (S row in
-//                registers, lazy maximum, a quarter of the exponentials on the
-//                FMA pipe, exp phases alternating between the groups)
+//   warps 8..15  softmax: one thread per row, a quarter of a row of S at a time;
+//                they also bring the next segment's queries (cp.async)
 // A key that a row does not see must not reach it.  Its S is replaced by -inf;
 // its value has the probability 0, and 0 times a value must be 0: slots past a
 // sequence's length are written as zeros, and a value group whose scale is NaN
@@ -35,7 +34,7 @@ namespace kv {
 namespace tc {
 
 constexpr int BQ = 128;
-constexpr int kRows = 2 * BQ;  // rows of an item
+constexpr int kRows = 2 * BQ;  // room for rows of an item (it has the whole query tokens that fit)
 constexpr int kKeys = 128;     // keys of a unit
 constexpr int kThreads = 512;
 constexpr int kLaunchRegs = 128;  // 65536 / 512
@@ -71,9 +70,7 @@ struct Segment {
   int more;            // another segment follows
   long long slot;      // of its part in the workspace, in rows
 };
-// Entries: warp 0 writes segment i + 8's when S of segment i + 5 is complete, by which
-// time every role is past segment i.  (It is written before the wait for a free query
-// buffer: the copies ahead of the conversion need it while that buffer is in use.)
+// Entries: one is written again when both softmax groups have seen its last P.V done.
 constexpr int kSegments = 8;
 
 template <int BITS>
@@ -84,8 +81,8 @@ struct Smem {
   uint8_t raw[4][Raw<BITS>::kStages][Raw<BITS>::kBytes];  // [warp]
   Flags flags[kFlags];
   Segment seg[kSegments];
-  uint64_t seg_full[kSegments];
-  uint64_t q_full[2], q_empty[2];
+  uint64_t seg_full[kSegments], seg_empty[kSegments];
+  uint64_t q_full[2][2];  // [buffer][group]
   uint64_t k_full[kRing], k_empty[kRing];
   uint64_t v_full[kRing], v_empty[kRing];
   uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
@@ -97,7 +94,7 @@ struct Smem {
 
 // Pages [0, count) of an item's span as units of two.
 __device__ __forceinline__ int units_of(const AttnParams& p, int group) {
-  return (span_of(p, group / p.row_blocks, group % p.row_blocks * kRows, kRows).count + 1) / 2;
+  return (span_of(p, group / p.row_blocks, group % p.row_blocks * p.block, p.block).count + 1) / 2;
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -194,8 +191,8 @@ __device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, 
 // A finished row of O_g: divided by its sum to the output, or as it is to the
 // CTA's part slot.  The caller has waited for the last P.V.
 __device__ __forceinline__ void finish_row(const AttnParams& p, uint32_t o_adr, float m, float l, uint32_t nan, int b,
-                                           int h, int ql, int row, bool whole, long long slot) {
-  const int rows = p.Lq * p.G, i = row / p.G, head = h * p.G + row - i * p.G;
+                                           int h, int ql, int row, bool there, bool whole, long long slot) {
+  const int i = row / p.G, head = h * p.G + row - i * p.G;
   const bool empty = i >= ql || l == 0.f;
   const float inv = !whole ? 1.f : empty ? 0.f : 1.f / l;
 #pragma unroll 1
@@ -206,7 +203,7 @@ __device__ __forceinline__ void finish_row(const AttnParams& p, uint32_t o_adr, 
 #pragma unroll
       for (int c = 0; c < HD / 2; ++c) o[c] = __uint_as_float(0x7FC00000u);
     }
-    if (row < rows) {
+    if (there) {
       if (whole) {
         uint4* dst = reinterpret_cast<uint4*>(p.o + (long long)b * p.o_batch + (long long)i * p.o_row +
                                               (long long)head * HD + half * (HD / 2));
@@ -225,7 +222,7 @@ __device__ __forceinline__ void finish_row(const AttnParams& p, uint32_t o_adr, 
       }
     }
   }
-  if (!whole && row < rows) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m, l);
+  if (!whole && there) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m, l);
 }
 
 __device__ __forceinline__ void tmem_start32(uint32_t a, uint32_t* r) {
@@ -259,7 +256,8 @@ __device__ __forceinline__ void tmem_put16(uint32_t a, const uint32_t* r) {
 __device__ __forceinline__ void tmem_put_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int BITS>
-__global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(AttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   Smem<BITS>& sm = *reinterpret_cast<Smem<BITS>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   volatile int* abort_flag = &sm.abort;
@@ -268,14 +266,17 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.q_full[i], 1);
-      mbar_init(&sm.q_empty[i], 2);
+      mbar_init(&sm.q_full[i][0], 4);
+      mbar_init(&sm.q_full[i][1], 4);
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.s_free[i], 128);
       mbar_init(&sm.p_full[i], 128);
       mbar_init(&sm.pv_done[i], 1);
     }
-    for (int s = 0; s < kSegments; ++s) mbar_init(&sm.seg_full[s], 1);
+    for (int s = 0; s < kSegments; ++s) {
+      mbar_init(&sm.seg_full[s], 1);
+      mbar_init(&sm.seg_empty[s], 2);
+    }
     for (int s = 0; s < kRing; ++s) {
       mbar_init(&sm.k_full[s], 4);
       mbar_init(&sm.k_empty[s], 2);
@@ -319,11 +320,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
     // rows that see nothing belong to no unit
 #pragma unroll 1
     for (int i = blockIdx.x; i < groups; i += gridDim.x) {
-      const int b = i / p.row_blocks, r0 = i % p.row_blocks * kRows;
+      const int b = i / p.row_blocks, r0 = i % p.row_blocks * p.block;
       if (units_of(p, i) > 0) continue;
 #pragma unroll 1
-      for (int x = threadIdx.x; x < heads * kRows * 8; x += kThreads) {
-        const int hh = x / (kRows * 8), row = r0 + (x >> 3) % kRows, qi = row / p.G;
+      for (int x = threadIdx.x; x < heads * p.block * 8; x += kThreads) {
+        const int hh = x / (p.block * 8), row = r0 + (x >> 3) % p.block, qi = row / p.G;
         if (row < rows)
           *reinterpret_cast<uint4*>(p.o + (long long)b * p.o_batch + (long long)qi * p.o_row +
                                     (long long)(hh * p.G + row - qi * p.G) * HD + (x & 7) * 8) = make_uint4(0, 0, 0, 0);
@@ -342,16 +343,20 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
     if (warp < 4) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
       if (warp == 0) {
-        // ---------------- segments and queries ----------------
+        // ---------------- segments ----------------
         int group = sm.group, units = units_of(p, group), h = sm.left / units, u0 = sm.left - h * units;
 #pragma unroll 1
         for (; ok && left > 0; ++it) {
-          const int b = group / p.row_blocks, r0 = (group - b * p.row_blocks) * kRows, qb = it & 1;
+          const int b = group / p.row_blocks, r0 = (group - b * p.row_blocks) * p.block;
           const int n = min(units - u0, left);
           left -= n;
+          if (it >= kSegments)
+            ok = mbar_wait_bounded(&sm.seg_empty[it % kSegments], ((it / kSegments) & 1) ^ 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           if (lane == 0) {
             Segment& sg = sm.seg[it % kSegments];
-            sg.sp = span_of(p, b, r0, kRows);
+            sg.sp = span_of(p, b, r0, p.block);
             sg.b = b;
             sg.h = h;
             sg.r0 = r0;
@@ -363,30 +368,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             mbar_arrive(&sm.seg_full[it % kSegments]);
             record_cut(p, d, group, h, u0, u0 + n, units, it);
           }
-          __syncwarp();
-          ok = mbar_wait_bounded(&sm.q_empty[qb], ((it >> 1) & 1) ^ 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const bf16* src = p.q + (long long)b * p.q_batch + (long long)h * p.G * HD + (lane & 7) * 8;
-          const uint32_t dst = smem_u32(sm.q[qb][0]);
-          int r = lane >> 3, i = (r0 + r) / p.G, hh = r0 + r - i * p.G;
-          const int di = 4 / p.G, dh = 4 - di * p.G;
-#pragma unroll 4
-          for (; r < kRows; r += 4) {
-            const bool there = r0 + r < rows;
-            const bf16* from = there ? src + (long long)i * p.q_row + hh * HD : p.q;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                             dst + r * 128 + (((lane & 7) ^ (r & 7)) << 4)),
-                         "l"(from), "r"(there ? 16 : 0)
-                         : "memory");
-            i += di;
-            hh += dh;
-            if (hh >= p.G) {
-              hh -= p.G;
-              ++i;
-            }
-          }
-          copy_commit();
           // the next item that has units
           u0 = 0;
           if (++h == heads && left > 0) {
@@ -395,10 +376,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             do units = units_of(p, ++group);
             while (units == 0);
           }
-          copy_wait<0>();
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.q_full[qb]);
         }
       } else if (warp < 3) {
         // ---------------- S issuers ----------------
@@ -412,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           if (!ok) break;
           const int n = sg.n, qb = it & 1;
           more = sg.more;
-          ok = mbar_wait_bounded(&sm.q_full[qb], (it >> 1) & 1, abort_flag);
+          ok = mbar_wait_bounded(&sm.q_full[qb][g], (it >> 1) & 1, abort_flag);
           const uint64_t qdesc = make_sw128_desc(smem_u32(sm.q[qb][g]));
 #pragma unroll 1
           for (int j = 0; ok && j < n; ++j, ++t) {
@@ -430,9 +407,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             }
             __syncwarp();
           }
-          if (!ok) break;
-          if (elect_one()) tc_commit(&sm.q_empty[qb]);
-          __syncwarp();
         }
       } else {
         // ---------------- P.V issuer ----------------
@@ -599,29 +573,59 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
       const uint32_t p_adr = tmem + lane_base + P_COL0 + (uint32_t)g * (kKeys / 2);
       const uint32_t o_adr = tmem + lane_base + O_COL0 + (uint32_t)g * HD;
       int t = 0;
-      // a segment's O_g is read out before the next one's first P_g is released
-      bool pending = false, pend_whole = false;
+      // a segment's O_g is read out before the next one's first P_g is released, so that
+      // its last P.V runs beside the next one's S
+      bool pending = false, pend_there = false, pend_whole = false;
       int pend_b = 0, pend_h = 0, pend_ql = 0, pend_row = 0;
       long long pend_slot = 0;
       float pend_m = 0.f, pend_l = 0.f;
       uint32_t pend_nan = 0;
+      // segment i's queries to their buffer: each warp its 32 rows, 4 rows an instruction
+      auto fetch_q = [&](int i) {
+        const Segment& sg = segment(i);
+        if (!ok) return;
+        const uint32_t dst = smem_u32(sm.q[i & 1][g]) + q * 4096;
+        const bf16* src = p.q + (long long)sg.b * p.q_batch + (long long)sg.h * p.G * HD + (lane & 7) * 8;
+        int row = sg.r0 + g * BQ + q * 32 + (lane >> 3), qi = row / p.G, hh = row - qi * p.G;
+        const int di = 4 / p.G, dh = 4 - di * p.G;
+#pragma unroll 1
+        for (int r = lane >> 3; r < 32; r += 4, row += 4) {
+          const bool there = row < rows;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           dst + r * 128 + (((lane & 7) ^ (r & 7)) << 4)),
+                       "l"(there ? src + (long long)qi * p.q_row + hh * HD : p.q), "r"(there ? 16 : 0)
+                       : "memory");
+          qi += di;
+          hh += dh;
+          if (hh >= p.G) {
+            hh -= p.G;
+            ++qi;
+          }
+        }
+        copy_commit();
+      };
+      auto post_q = [&](int i) {
+        copy_wait<0>();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[i & 1][g]);
+      };
+      fetch_q(0);
+      post_q(0);
 #pragma unroll 1
       for (bool more = true; ok; ++it) {
-        if (pending) {
-          ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_whole, pend_slot);
-        }
         if (!more) break;
         const Segment& sg = segment(it);
         if (!ok) break;
         more = sg.more;
+        // (the buffer's last reader, S of the segment before, is done)
+        if (more) fetch_q(it + 1);
+        if (!ok) break;
         const Span sp = sg.sp;
         const int u0 = sg.u0, n = sg.n, r0 = sg.r0;
         const int row = r0 + g * BQ + q * 32 + lane, i = row / p.G;
-        const int pos = row < rows && i < sp.ql ? sp.pos(i, p.causal) : -1;
+        const bool mine = row < rows && row < r0 + p.block;
+        const int pos = mine && i < sp.ql ? sp.pos(i, p.causal) : -1;
         const bool idle = r0 + g * BQ + q * 32 >= rows;  // no row in this warp
         float m = -INFINITY, l = 0.f;
         uint32_t nan = 0;
@@ -677,25 +681,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             for (int c = 0; c < 32; c += 2) {
               float x0, x1, e0, e1;
               attn_tc::fma2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]), p.scale_log2, -mbase, x0, x1);
-              if (((c >> 1) & 7) < 2) {
-                attn_tc::ex2_poly2(x0, x1, e0, e1);
-              } else {
-                e0 = ex2(x0);
-                e1 = ex2(x1);
-              }
+              e0 = ex2(x0);
+              e1 = ex2(x1);
               attn_tc::add2(rs[c & 2], rs[(c & 2) + 1], e0, e1);
               pk[c >> 1] = pack_bf16x2(e0, e1);
-            }
-            if (!plain) {  // the polynomial ends at 2^-126: a key that is not seen gives 0
-              const uint32_t v = qt == 0 ? vis[0] : qt == 1 ? vis[1] : qt == 2 ? vis[2] : vis[3];
-#pragma unroll
-              for (int c = 0; c < 32; c += 16) {  // the pairs that took it
-#pragma unroll
-                for (int e = c; e < c + 4; e += 2) {
-                  const uint32_t two = v >> e;
-                  pk[e >> 1] &= ((two & 1u) ? 0x0000FFFFu : 0u) | ((two & 2u) ? 0xFFFF0000u : 0u);
-                }
-              }
             }
             tmem_put16(p_adr + qt * 16, pk);
           };
@@ -707,58 +696,63 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             if (!ok) break;
             tc_fence_after();
           }
+          if (j == 0 && pending) {
+            if (q == 0 && lane == 0) mbar_arrive(&sm.seg_empty[(it - 1) % kSegments]);
+            finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_there, pend_whole, pend_slot);
+          }
           if (!idle) {
-            bool again = j == 0;
-            if (!again) {
+            if (j == 0) {  // no maximum yet: the unit's own, first
 #pragma unroll 1
               for (int qt = 0; qt < 4; qt += 2) {
                 tmem_wait32(sa[0]);
                 tmem_start32(s_adr + 32 * qt + 32, sa[1]);
                 mask(sa[0], qt);
                 top(sa[0]);
-                exps(sa[0], qt);
                 tmem_wait32(sa[1]);
-                if (qt == 0) tmem_start32(s_adr + 64, sa[0]);
+                tmem_start32(s_adr + (qt == 0 ? 64 : 0), sa[0]);
                 mask(sa[1], qt + 1);
                 top(sa[1]);
-                if (qt == 2) {
-                  const float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-                  again = __any_sync(0xffffffffu, mx > m + kRescaleLog2);
-                  if (!again) {
-                    tc_fence_before();
-                    mbar_arrive(&sm.s_free[g]);
-                  }
-                }
-                exps(sa[1], qt + 1);
               }
-            } else {
+              m = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+            }
+            bool again = false;
+            float mx = m;
+#pragma unroll 1
+            for (int qt = 0; qt < 4; qt += 2) {
               tmem_wait32(sa[0]);
+              tmem_start32(s_adr + 32 * qt + 32, sa[1]);
+              mask(sa[0], qt);
+              top(sa[0]);
+              exps(sa[0], qt);
+              tmem_wait32(sa[1]);
+              if (qt == 0) tmem_start32(s_adr + 64, sa[0]);
+              mask(sa[1], qt + 1);
+              top(sa[1]);
+              if (qt == 2) {
+                mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+                again = __any_sync(0xffffffffu, mx > m + kRescaleLog2);
+                if (!again) {
+                  tc_fence_before();
+                  mbar_arrive(&sm.s_free[g]);
+                }
+              }
+              exps(sa[1], qt + 1);
             }
             if (again) {
-#pragma unroll 1
-              for (int qt = 0; qt < 4; ++qt) {
-                tmem_start32(s_adr + 32 * qt, sa[0]);
-                tmem_wait32(sa[0]);
-                mask(sa[0], qt);
-                top(sa[0]);
-              }
-              const float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
               float alpha = 1.f;
               if (mx > m + kRescaleLog2) {
                 alpha = ex2(m - mx);
                 m = mx;
                 l *= alpha;
               }
-              if (j > 0) {
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 16) {
-                  float o[16];
-                  uint32_t u[16];
-                  tmem_ld16(o_adr + c, o);
+              for (int c = 0; c < HD; c += 16) {
+                float o[16];
+                uint32_t u[16];
+                tmem_ld16(o_adr + c, o);
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
-                  attn_tc::tmem_st16(o_adr + c, u);
-                }
+                for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
+                attn_tc::tmem_st16(o_adr + c, u);
               }
 #pragma unroll
               for (int e = 0; e < 4; ++e) rs[e] = 0.f;
@@ -777,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
             }
             tmem_put_wait();
             const float sum = (rs[0] + rs[1]) + (rs[2] + rs[3]);
-            l += m == -INFINITY && sum == sum ? 0.f : sum;  // no key seen yet: the polynomial's 2^-126 do not count
+            l += sum;
           } else {
             tc_fence_before();
             mbar_arrive(&sm.s_free[g]);
@@ -786,10 +780,19 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(AttnParams p) {
           mbar_arrive(&sm.p_full[g]);
         }
         if (!ok) break;
+        if (more) post_q(it + 1);
         pending = true;
         pend_whole = sg.whole != 0;
-        pend_b = sg.b, pend_h = sg.h, pend_ql = sp.ql, pend_row = row, pend_m = m, pend_l = l, pend_nan = nan;
+        pend_b = sg.b, pend_h = sg.h, pend_ql = sp.ql, pend_row = row, pend_there = mine, pend_m = m, pend_l = l, pend_nan = nan;
         pend_slot = sg.slot + (row - r0);
+      }
+      if (ok && pending) {
+        ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          tc_fence_after();
+          finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_there, pend_whole, pend_slot);
+        }
       }
     }
     if (!ok && lane == 0) {

@@ -96,6 +96,7 @@ static int read(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, 
 struct Plan {
   int nt;          // 8-row tiles of the mma.sync kernel, 0: the tcgen05 kernel
   int block, row_blocks, split;  // rows of a block, blocks per (sequence, kv head)
+  int slots;       // rows of a part in the workspace
   size_t workspace;
 };
 
@@ -126,6 +127,7 @@ static int resident_ctas(int bits, int nt) {
 static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a, Plan* out) {
   const long long rows = (long long)a->Lq * (a->Hq / c->kv_heads);
   VLA_CHECK_ARG(rows < (1ll << 30), "kv_attention: too many query rows");
+  const int G = a->Hq / c->kv_heads;
   out->nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
   const int block = out->nt > 0 ? 8 * out->nt : tc::kRows;
   const long long blocks = (rows + block - 1) / block;
@@ -133,16 +135,17 @@ static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a,
   long long keys = a->max_len > 0 && a->max_len < room ? a->max_len : room;
   if (a->window > 0) {
     // the window of a block's rows and the first tokens, in whole pages
-    const long long seen = (long long)a->window + a->sinks + (block - 1) / (a->Hq / c->kv_heads) + 3 * kUnit;
+    const long long seen = (long long)a->window + a->sinks + (block - 1) / G + 3 * kUnit;
     if (seen < keys) keys = seen;
   }
   VLA_CHECK_ARG(c->batch * blocks * c->kv_heads <= ((1ll << 31) - 1) / (c->max_pages > 0 ? c->max_pages : 1) && c->batch * rows * c->kv_heads < (1ll << 31),
                 "kv_attention: too many work items");
   out->block = block;
+  out->slots = out->nt > 0 ? block : tc::kRows;
   out->row_blocks = (int)blocks;
   out->split = out->nt == 0 || keys > 8 * kUnit;
   const size_t ctas = out->nt == 0 ? device_info().num_sms : out->split ? resident_ctas(c->bits, out->nt) : 0;
-  out->workspace = ctas * (2 * block * (HD + 2) * sizeof(float) + sizeof(int4));
+  out->workspace = ctas * (2 * out->slots * (HD + 2) * sizeof(float) + sizeof(int4));
   return VLA_OK;
 }
 
@@ -186,7 +189,7 @@ static int launch_tc(const AttnParams& p, cudaStream_t st) {
   }
   const int ctas = device_info().num_sms;
   launch_k(tc::attend_kernel<BITS>, dim3(ctas), dim3(tc::kThreads), smem, st, p);
-  const int slices = ((p.row_blocks > 1 ? tc::kRows : p.Lq * p.G) + kJoinWarps - 1) / kJoinWarps;
+  const int slices = ((p.row_blocks > 1 ? p.block : p.Lq * p.G) + kJoinWarps - 1) / kJoinWarps;
   launch_k(join_kernel<tc::kRows, 1>, dim3(slices, ctas), dim3(kJoinWarps * 32), 0, st, p, 1.f);
   return VLA_OK;
 }
@@ -231,11 +234,12 @@ static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cuda
   p.sinks = a->sinks < room ? a->sinks : (int)room;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.mask = c->bits == 4 ? code_mask<4>() : code_mask<8>();
+  p.block = pl.block;
   p.row_blocks = pl.row_blocks;
   p.split = pl.split;
   p.part_o = (float*)a->workspace;
   if (pl.split) {
-    const size_t rows = pl.workspace / (2 * pl.block * (HD + 2) * sizeof(float) + sizeof(int4)) * 2 * pl.block;
+    const size_t rows = pl.workspace / (2 * pl.slots * (HD + 2) * sizeof(float) + sizeof(int4)) * 2 * pl.slots;
     p.part_ml = p.part_o + rows * HD;
     p.cut = reinterpret_cast<int4*>(p.part_ml + rows * 2);
   }
