@@ -10,16 +10,22 @@
 // windows and uneven lengths leave no SM waiting; an item cut by a CTA's border
 // leaves fp32 sums that join_kernel adds.  Warp roles:
 //   warp 0       the CTA's segments (shares of items), for the other roles
-//   warps 1, 2   S issuers, one per group: S_g = Q_g K^T (128 x 128 into TMEM)
-//   warp 3       P.V issuer: O_g += P_g V (P from TMEM, V as the MN-major operand)
+//   warp 1       S issuer: S = Q_g K^T (128 x 128), unit by unit, group 0 then 1, into
+//                three TMEM buffers in turn: it runs ahead of the softmax
+//   warp 2       P.V issuer in the same order: O_g += P V (P from TMEM, where its S was;
+//                V as the MN-major operand)
 //   warps 4..7   codes to bf16: each takes 32 keys of the unit, copies their codes
 //                and scales two units ahead (cp.async into a ring of its own) and
 //                writes code * scale, exact in bf16, into the swizzled K and V
 //                rings.  Against a bf16 cache this is what the kernel adds: about
 //                320 instructions per thread and unit beside the softmax's 2000
 //                issue slots.
-//   warps 8..15  softmax: one thread per row, a quarter of a row of S at a time;
-//                they also bring the next segment's queries (cp.async)
+//   warps 8..23  softmax: two threads per row, each 64 of a unit's 128 keys (one
+//                page), which tell each other their maxima; they also bring the next
+//                segment's queries (cp.async).  Sixteen warps, because one warp's
+//                chain of TMEM loads, exponentials and packing, not any pipe, is what
+//                a unit waits for: with one thread per row (eight warps) 1024 rows over
+//                4 x 8192 keys took 190 us.
 // A key that a row does not see must not reach it.  Its S is replaced by -inf;
 // its value has the probability 0, and 0 times a value must be 0: slots past a
 // sequence's length are written as zeros, and a value group whose scale is NaN
@@ -36,16 +42,17 @@ namespace tc {
 constexpr int BQ = 128;
 constexpr int kRows = 2 * BQ;  // room for rows of an item (it has the whole query tokens that fit)
 constexpr int kKeys = 128;     // keys of a unit
-constexpr int kThreads = 512;
-constexpr int kLaunchRegs = 128;  // 65536 / 512
-constexpr int kIssueRegs = 88;    // warps 0..3
-constexpr int kCodeRegs = 88;     // warps 4..7
-constexpr int kSoftRegs = 168;    // warps 8..15
-static_assert(kIssueRegs + kCodeRegs + 2 * kSoftRegs == 4 * kLaunchRegs, "register split must equal the launch total");
+constexpr int kThreads = 768;
+constexpr int kLaunchRegs = 80;  // 65536 / 768, rounded down to a multiple of 8
+constexpr int kIssueRegs = 56;   // warps 0..3
+constexpr int kCodeRegs = 72;    // warps 4..7
+constexpr int kSoftRegs = 88;    // warps 8..23
+static_assert(kIssueRegs + kCodeRegs + 4 * kSoftRegs == 6 * kLaunchRegs, "register split must equal the launch total");
 constexpr int kRing = 3;    // K and V tiles
 constexpr int kFlags = 4;   // flag sets: a softmax thread reads set j before S(j+1) may be issued
 constexpr int TILE_BYTES = kKeys * HD * 2;
-constexpr uint32_t S_COL0 = 0, P_COL0 = 256, O_COL0 = 384;
+constexpr int kBuffers = 3;  // S and P of a tile (unit t, group g) in buffer (2 t + g) % 3
+constexpr uint32_t O_COL0 = kBuffers * kKeys;
 constexpr float kRescaleLog2 = 8.f;
 
 // What a converting warp copies: half a page.
@@ -56,9 +63,9 @@ struct Raw {
   static constexpr int kStages = 3;
 };
 
-struct Flags {
-  uint32_t nan[2][4];  // per value group: keys whose scale is NaN
-  uint32_t absent[4];  // per 32 keys: not there
+struct Flags {              // per page of a unit
+  uint32_t nan[2][4];       // keys whose value scale is NaN: [group 0: 32 keys, 32 keys, group 1: 32, 32]
+  uint32_t absent[2][2];    // per 32 keys: not there
 };
 
 // A CTA's share of an item, as warp 0 hands it to the other roles.
@@ -85,7 +92,9 @@ struct Smem {
   uint64_t q_full[2][2];  // [buffer][group]
   uint64_t k_full[kRing], k_empty[kRing];
   uint64_t v_full[kRing], v_empty[kRing];
-  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
+  uint64_t s_full[kBuffers], s_empty[kBuffers];  // per buffer
+  uint64_t p_full[2], pv_done[2];                // per group
+  float2 swap[2][2][kRows];    // [turn][half of the keys]: what they tell each other
   int scan[kThreads / 32];
   int group, left;
   uint32_t tmem_base;
@@ -188,41 +197,35 @@ __device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, 
   }
 }
 
-// A finished row of O_g: divided by its sum to the output, or as it is to the
-// CTA's part slot.  The caller has waited for the last P.V.
-__device__ __forceinline__ void finish_row(const AttnParams& p, uint32_t o_adr, float m, float l, uint32_t nan, int b,
-                                           int h, int ql, int row, bool there, bool whole, long long slot) {
-  const int i = row / p.G, head = h * p.G + row - i * p.G;
-  const bool empty = i >= ql || l == 0.f;
-  const float inv = !whole ? 1.f : empty ? 0.f : 1.f / l;
-#pragma unroll 1
-  for (int half = 0; half < 2; ++half) {
-    float o[HD / 2];
-    tmem_ld32(o_adr + (uint32_t)half * (HD / 2), o);  // warp-collective: every lane loads
-    if ((nan >> half) & 1u) {
+// Where a thread's half of a finished row goes, and what it is divided by.
+struct Pending {
+  bf16* out;      // the output's 32 dims, or
+  float* part;    // the part slot's
+  float2* ml;     // ... and its maximum and sum, from one of the two threads
+  float m, l;
+  uint32_t nan;
+  bool none;      // the query token is not there: zeros
+};
+
+// 32 dims of a finished row of O_g.  The caller has waited for the last P.V, and l
+// and nan are the whole row's.
+__device__ __forceinline__ void finish_row(const Pending& d, uint32_t o_adr, float l, bool nan) {
+  const bool zero = d.none || (l == 0.f && !nan);
+  const float inv = 1.f / l;
+  float o[HD / 2];
+  tmem_ld32(o_adr, o);  // warp-collective: every lane loads
+  if (d.out != nullptr) {
 #pragma unroll
-      for (int c = 0; c < HD / 2; ++c) o[c] = __uint_as_float(0x7FC00000u);
-    }
-    if (there) {
-      if (whole) {
-        uint4* dst = reinterpret_cast<uint4*>(p.o + (long long)b * p.o_batch + (long long)i * p.o_row +
-                                              (long long)head * HD + half * (HD / 2));
+    for (int c = 0; c < HD / 2; ++c) o[c] = zero ? 0.f : nan ? __uint_as_float(0x7FC00000u) : o[c] * inv;
 #pragma unroll
-        for (int c8 = 0; c8 < HD / 16; ++c8) {
-          float tv8[8];
+    for (int c = 0; c < HD / 2; c += 8) *reinterpret_cast<uint4*>(d.out + c) = pack_bf16x8(o + c);
+  } else if (d.part != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) tv8[e] = empty && !((nan >> half) & 1u) ? 0.f : o[c8 * 8 + e] * inv;
-          dst[c8] = pack_bf16x8(tv8);
-        }
-      } else {
-        float4* dst = reinterpret_cast<float4*>(p.part_o + slot * HD + half * (HD / 2));
-#pragma unroll
-        for (int c4 = 0; c4 < HD / 8; ++c4)
-          dst[c4] = make_float4(o[4 * c4], o[4 * c4 + 1], o[4 * c4 + 2], o[4 * c4 + 3]);
-      }
-    }
+    for (int c = 0; c < HD / 2; c += 4)
+      *reinterpret_cast<float4*>(d.part + c) =
+          nan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+    if (d.ml != nullptr) *d.ml = make_float2(d.m, l);
   }
-  if (!whole && there) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m, l);
 }
 
 __device__ __forceinline__ void tmem_start32(uint32_t a, uint32_t* r) {
@@ -266,12 +269,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.q_full[i][0], 4);
-      mbar_init(&sm.q_full[i][1], 4);
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.s_free[i], 128);
-      mbar_init(&sm.p_full[i], 128);
+      mbar_init(&sm.q_full[i][0], 8);
+      mbar_init(&sm.q_full[i][1], 8);
+      mbar_init(&sm.p_full[i], 256);
       mbar_init(&sm.pv_done[i], 1);
+    }
+    for (int i = 0; i < kBuffers; ++i) {
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.s_empty[i], 1);
     }
     for (int s = 0; s < kSegments; ++s) {
       mbar_init(&sm.seg_full[s], 1);
@@ -279,9 +284,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < kRing; ++s) {
       mbar_init(&sm.k_full[s], 4);
-      mbar_init(&sm.k_empty[s], 2);
+      mbar_init(&sm.k_empty[s], 1);
       mbar_init(&sm.v_full[s], 4);
-      mbar_init(&sm.v_empty[s], 2);
+      mbar_init(&sm.v_empty[s], 1);
     }
     sm.abort = 0;
     mbar_fence_init();
@@ -344,10 +349,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
       if (warp == 0) {
         // ---------------- segments ----------------
-        int group = sm.group, units = units_of(p, group), h = sm.left / units, u0 = sm.left - h * units;
+        int group = sm.group - 1, h = heads, u0 = 0, units = 0;
+        Span sp;
 #pragma unroll 1
         for (; ok && left > 0; ++it) {
-          const int b = group / p.row_blocks, r0 = (group - b * p.row_blocks) * p.block;
+          if (h == heads) {  // the next group that has units
+#pragma unroll 1
+            do {
+              ++group;
+              sp = span_of(p, group / p.row_blocks, group % p.row_blocks * p.block, p.block);
+              units = (sp.count + 1) / 2;
+            } while (units == 0);
+            h = 0;
+            if (it == 0) {
+              h = sm.left / units;
+              u0 = sm.left - h * units;
+            }
+          }
           const int n = min(units - u0, left);
           left -= n;
           if (it >= kSegments)
@@ -356,32 +374,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           if (lane == 0) {
             Segment& sg = sm.seg[it % kSegments];
-            sg.sp = span_of(p, b, r0, p.block);
-            sg.b = b;
+            sg.sp = sp;
+            sg.b = group / p.row_blocks;
             sg.h = h;
-            sg.r0 = r0;
+            sg.r0 = group % p.row_blocks * p.block;
             sg.u0 = u0;
             sg.n = n;
             sg.whole = n == units;
             sg.more = left > 0;
             sg.slot = (2ll * blockIdx.x + (it > 0 ? 1 : 0)) * kRows;
             mbar_arrive(&sm.seg_full[it % kSegments]);
-            record_cut(p, d, group, h, u0, u0 + n, units, it);
+            if (left == 0) record_cut(p, d, group, h, u0, u0 + n, units, it);
           }
-          // the next item that has units
           u0 = 0;
-          if (++h == heads && left > 0) {
-            h = 0;
-#pragma unroll 1
-            do units = units_of(p, ++group);
-            while (units == 0);
-          }
+          ++h;
         }
-      } else if (warp < 3) {
-        // ---------------- S issuers ----------------
-        const int g = warp - 1;
+      } else if (warp == 1) {
+        // ---------------- S issuer: group 0's tile, then group 1's ----------------
         constexpr uint32_t idesc_s = make_idesc_bf16(BQ, kKeys);
-        const uint32_t s_tmem = tmem + S_COL0 + (uint32_t)g * kKeys;
         int t = 0;
 #pragma unroll 1
         for (bool more = true; more && ok; ++it) {
@@ -389,27 +399,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           const int n = sg.n, qb = it & 1;
           more = sg.more;
-          ok = mbar_wait_bounded(&sm.q_full[qb][g], (it >> 1) & 1, abort_flag);
-          const uint64_t qdesc = make_sw128_desc(smem_u32(sm.q[qb][g]));
 #pragma unroll 1
-          for (int j = 0; ok && j < n; ++j, ++t) {
-            const int sk = t % kRing;
-            ok = mbar_wait_bounded(&sm.k_full[sk], (t / kRing) & 1, abort_flag);
-            if (ok && t > 0) ok = mbar_wait_bounded(&sm.s_free[g], (uint32_t)(t - 1) & 1u, abort_flag);
+          for (int j = 0; ok && j < 2 * n; ++j) {
+            const int tile = 2 * t + j, g = j & 1, buf = tile % kBuffers, sk = (tile >> 1) % kRing;
+            if (j < 2) ok = mbar_wait_bounded(&sm.q_full[qb][g], (it >> 1) & 1, abort_flag);
+            if (ok) ok = mbar_wait_bounded(&sm.k_full[sk], ((tile >> 1) / kRing) & 1, abort_flag);
+            if (ok) ok = mbar_wait_bounded(&sm.s_empty[buf], ((tile / kBuffers) & 1) ^ 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
+              const uint64_t qdesc = make_sw128_desc(smem_u32(sm.q[qb][g]));
               const uint64_t kdesc = make_sw128_desc(smem_u32(sm.k[sk]));
 #pragma unroll
-              for (int k = 0; k < HD / 16; ++k) tc_mma_bf16(s_tmem, qdesc + 2 * k, kdesc + 2 * k, idesc_s, k > 0);
-              tc_commit(&sm.s_full[g]);
-              tc_commit(&sm.k_empty[sk]);
+              for (int k = 0; k < HD / 16; ++k)
+                tc_mma_bf16(tmem + (uint32_t)(buf * kKeys), qdesc + 2 * k, kdesc + 2 * k, idesc_s, k > 0);
+              tc_commit(&sm.s_full[buf]);
+              if (g == 1) tc_commit(&sm.k_empty[sk]);
             }
             __syncwarp();
           }
+          t += n;
         }
-      } else {
-        // ---------------- P.V issuer ----------------
+      } else if (warp == 2) {
+        // ---------------- P.V issuer, in the same order ----------------
         constexpr uint32_t idesc_pv = make_idesc_bf16(BQ, HD) | (1u << 16);  // B (V) is MN-major
         int t = 0;
 #pragma unroll 1
@@ -419,29 +431,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int n = sg.n;
           more = sg.more;
 #pragma unroll 1
-          for (int j = 0; ok && j < n; ++j, ++t) {
-            const int sv = t % kRing;
-#pragma unroll 1
-            for (int g = 0; g < 2; ++g) {
-              ok = mbar_wait_bounded(&sm.p_full[g], (uint32_t)t & 1u, abort_flag);
-              if (ok) ok = mbar_wait_bounded(&sm.v_full[sv], (t / kRing) & 1, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-              if (elect_one()) {
-                const uint32_t p_tmem = tmem + P_COL0 + (uint32_t)g * (kKeys / 2);
-                const uint32_t o_tmem = tmem + O_COL0 + (uint32_t)g * HD;
-                const uint32_t vbase = smem_u32(sm.v[sv]);
+          for (int j = 0; ok && j < 2 * n; ++j) {
+            const int tile = 2 * t + j, g = j & 1, buf = tile % kBuffers, sv = (tile >> 1) % kRing;
+            ok = mbar_wait_bounded(&sm.p_full[g], (uint32_t)(tile >> 1) & 1u, abort_flag);
+            if (ok) ok = mbar_wait_bounded(&sm.v_full[sv], ((tile >> 1) / kRing) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t p_tmem = tmem + (uint32_t)(buf * kKeys), o_tmem = tmem + O_COL0 + (uint32_t)(g * HD);
+              const uint32_t vbase = smem_u32(sm.v[sv]);
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                  attn_tc::tc_mma_bf16_ts(o_tmem, p_tmem + (uint32_t)k * 8u,
-                                          attn_tc::make_sw128_mn_desc(vbase + (uint32_t)k * 2048u, 16384u), idesc_pv,
-                                          (j > 0 || k > 0) ? 1u : 0u);
-                tc_commit(&sm.pv_done[g]);
-                tc_commit(&sm.v_empty[sv]);
-              }
-              __syncwarp();
+              for (int k = 0; k < kKeys / 16; ++k)  // 16 keys; P of 32 keys lies where their S began
+                attn_tc::tc_mma_bf16_ts(o_tmem, p_tmem + (uint32_t)((k >> 1) * 32 + (k & 1) * 8),
+                                        attn_tc::make_sw128_mn_desc(vbase + (uint32_t)k * 2048u, 16384u), idesc_pv,
+                                        (j > 1 || k > 0) ? 1u : 0u);
+              tc_commit(&sm.pv_done[g]);
+              tc_commit(&sm.s_empty[buf]);
+              if (g == 1) tc_commit(&sm.v_empty[sv]);
             }
+            __syncwarp();
           }
+          t += n;
         }
       }
     } else if (warp < 8) {
@@ -450,39 +460,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       using Rw = Raw<BITS>;
       const int w = warp - 4;  // keys [32 w, 32 w + 32) of a unit: half (w & 1) of page w >> 1
       const uint32_t raw = smem_u32(sm.raw[w]);
-      // copies run kStages - 1 units ahead, with a segment count of their own
-      int ci = 0, cu = 0, cn = 0, ct = 0, cpage = 0, cb = 0, ch = 0;
-      int csink = 0, cfirst = 0, ccount = 0;
-      bool cmore = true;
+      // step c copies unit c and converts unit c - kStages + 1, each with a segment of its own
+      int ci = 0, cu = 0, cn = 0, cb = 0, ch = 0, csink = 0, cfirst = 0, ccount = 0;
+      int u0 = 0, n = 0, j = 0, len = 0, sink = 0, first = 0;
+      bool cmore = true, more = true;
       uint32_t there = 0;  // bit (stage): the page exists
-      auto page_ahead = [&]() {  // the next copy's page number
-        const int u = 2 * cu + (w >> 1);
-        if (u < ccount) cpage = p.c.table[(long long)cb * p.c.table_ld + (u < csink ? u : cfirst + u - csink)];
-      };
-      auto copy_segment = [&]() {
-        const Segment& sg = segment(ci);
-        ++ci;
-        if (!ok) return;
-        cu = sg.u0;
-        cn = sg.n;
-        cb = sg.b;
-        ch = sg.h;
-        csink = sg.sp.sink;
-        cfirst = sg.sp.first;
-        ccount = sg.sp.count;
-        cmore = sg.more;
-        page_ahead();
-      };
-      copy_segment();
-      auto copy_next = [&]() {
-        if (cn == 0 && cmore) copy_segment();
-        if (cn > 0 && ok) {
-          const int st = ct % Rw::kStages, u = 2 * cu + (w >> 1);
+#pragma unroll 1
+      for (int c = 0; ok; ++c) {
+        const bool there_now = (there >> ((c + 1) % Rw::kStages)) & 1u;  // of the unit to convert
+        if (cn == 0 && cmore) {
+          const Segment& sg = segment(ci++);
+          if (!ok) break;
+          cu = sg.u0;
+          cn = sg.n;
+          cb = sg.b;
+          ch = sg.h;
+          csink = sg.sp.sink;
+          cfirst = sg.sp.first;
+          ccount = sg.sp.count;
+          cmore = sg.more;
+        }
+        if (cn > 0) {
+          const int st = c % Rw::kStages, u = 2 * cu + (w >> 1);
           bool have = false;
           if (u < ccount) {
-            have = cpage >= 0 && cpage < p.c.pages;
+            const int page = p.c.table[(long long)cb * p.c.table_ld + (u < csink ? u : cfirst + u - csink)];
+            have = page >= 0 && page < p.c.pages;
             if (have) {
-              const uint8_t* blk = p.c.pool + ((long long)cpage * heads + ch) * Block<BITS>::kBytes;
+              const uint8_t* blk = p.c.pool + ((long long)page * heads + ch) * Block<BITS>::kBytes;
               const uint32_t dst = raw + st * Rw::kBytes + lane * 16;
               const uint8_t* src = blk + (w & 1) * Rw::kCodes + lane * 16;
 #pragma unroll
@@ -497,35 +502,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           there = have ? there | (1u << st) : there & ~(1u << st);
-          ++ct;
           ++cu;
-          if (--cn > 0)
-            page_ahead();
-          else if (cmore && __all_sync(0xffffffffu, mbar_test(&sm.seg_full[ci % kSegments], (ci / kSegments) & 1)))
-            copy_segment();
+          --cn;
         }
         copy_commit();
-      };
-#pragma unroll
-      for (int i = 0; i < Rw::kStages - 1; ++i) copy_next();
-      int t = 0;
-#pragma unroll 1
-      for (bool more = ok; more && ok; ++it) {
-        const Segment& sg = segment(it);
-        if (!ok) break;
-        const int n = sg.n, u0 = sg.u0, len = sg.sp.len, sink = sg.sp.sink, first = sg.sp.first;
-        more = sg.more;
-#pragma unroll 1
-        for (int j = 0; ok && j < n; ++j, ++t) {
-          const int st = t % Rw::kStages, sr = t % kRing;
-          const bool have = (there >> st) & 1u;  // before copy_next changes another stage's bit
-          copy_next();
-          copy_wait<Rw::kStages - 1>();
-          __syncwarp();
-          ok = mbar_wait_bounded(&sm.k_empty[sr], ((t / kRing) & 1) ^ 1, abort_flag);
-          if (ok) ok = mbar_wait_bounded(&sm.v_empty[sr], ((t / kRing) & 1) ^ 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+        const int t = c - (Rw::kStages - 1);
+        if (t < 0) continue;
+        if (j == n) {
+          if (!more) break;
+          const Segment& sg = segment(it++);
           if (!ok) break;
+          n = sg.n;
+          u0 = sg.u0;
+          len = sg.sp.len;
+          sink = sg.sp.sink;
+          first = sg.sp.first;
+          more = sg.more;
+          j = 0;
+        }
+        const int st = t % Rw::kStages, sr = t % kRing;
+        const bool have = there_now;
+        copy_wait<Rw::kStages - 1>();
+        __syncwarp();
+        ok = mbar_wait_bounded(&sm.k_empty[sr], ((t / kRing) & 1) ^ 1, abort_flag);
+        if (ok) ok = mbar_wait_bounded(&sm.v_empty[sr], ((t / kRing) & 1) ^ 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
           const uint32_t kt = smem_u32(sm.k[sr]), vt = smem_u32(sm.v[sr]), from = raw + st * Rw::kBytes;
           const int u = 2 * (u0 + j) + (w >> 1), page = u < sink ? u : first + u - sink;
           int live = 0;  // of the 32 keys, those inside the sequence
@@ -551,9 +553,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (lane == 0) {
             Flags& f = sm.flags[t % kFlags];
-            f.nan[0][w] = n0;
-            f.nan[1][w] = n1;
-            f.absent[w] = have ? 0u : 1u;
+            f.nan[w >> 1][w & 1] = n0;
+            f.nan[w >> 1][2 + (w & 1)] = n1;
+            f.absent[w >> 1][w & 1] = have ? 0u : 1u;
           }
           fence_async_smem();
           __syncwarp();
@@ -561,238 +563,217 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(&sm.k_full[sr]);
             mbar_arrive(&sm.v_full[sr]);
           }
-        }
+        ++j;
       }
       copy_wait<0>();
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
       // ---------------- softmax / output ----------------
-      const int g = (warp - 8) >> 2, q = warp & 3;
+      const int g = (warp - 8) >> 3, hf = (warp >> 2) & 1, q = warp & 3;  // query tile, half of the keys, lane quarter
       const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-      const uint32_t s_adr = tmem + lane_base + S_COL0 + (uint32_t)g * kKeys;
-      const uint32_t p_adr = tmem + lane_base + P_COL0 + (uint32_t)g * (kKeys / 2);
-      const uint32_t o_adr = tmem + lane_base + O_COL0 + (uint32_t)g * HD;
-      int t = 0;
-      // a segment's O_g is read out before the next one's first P_g is released, so that
-      // its last P.V runs beside the next one's S
-      bool pending = false, pend_there = false, pend_whole = false;
-      int pend_b = 0, pend_h = 0, pend_ql = 0, pend_row = 0;
-      long long pend_slot = 0;
-      float pend_m = 0.f, pend_l = 0.f;
-      uint32_t pend_nan = 0;
-      // segment i's queries to their buffer: each warp its 32 rows, 4 rows an instruction
-      auto fetch_q = [&](int i) {
-        const Segment& sg = segment(i);
-        if (!ok) return;
-        const uint32_t dst = smem_u32(sm.q[i & 1][g]) + q * 4096;
-        const bf16* src = p.q + (long long)sg.b * p.q_batch + (long long)sg.h * p.G * HD + (lane & 7) * 8;
-        int row = sg.r0 + g * BQ + q * 32 + (lane >> 3), qi = row / p.G, hh = row - qi * p.G;
-        const int di = 4 / p.G, dh = 4 - di * p.G;
+      const uint32_t s_adr0 = tmem + lane_base + (uint32_t)(hf * kUnit);
+      const uint32_t o_adr = tmem + lane_base + O_COL0 + (uint32_t)(g * HD + hf * (HD / 2));
+      int t = 0, turn = 0;
+      // Tells the row's other thread (v, bits), returns what it tells.  The two warps meet
+      // at a named barrier; one that gives up arrives there (below), so none is left waiting.
+      auto swap = [&](float v, uint32_t bits) {
+        const int at = g * BQ + q * 32 + lane;
+        sm.swap[turn & 1][hf][at] = make_float2(v, __uint_as_float(bits));
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+        float2 r;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(r.x), "=f"(r.y)
+                     : "r"(smem_u32(&sm.swap[turn & 1][hf ^ 1][at])));
+        ++turn;
+        if (*abort_flag) ok = false;  // (raised before the other warp gave up)
+        return r;
+      };
+      // what the last segment's rows are finished with, once its last P.V is done
+      Pending pend{};
+      bool pend_idle = true;
+      bool more = true;
 #pragma unroll 1
-        for (int r = lane >> 3; r < 32; r += 4, row += 4) {
-          const bool there = row < rows;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                           dst + r * 128 + (((lane & 7) ^ (r & 7)) << 4)),
-                       "l"(there ? src + (long long)qi * p.q_row + hh * HD : p.q), "r"(there ? 16 : 0)
-                       : "memory");
-          qi += di;
-          hh += dh;
-          if (hh >= p.G) {
-            hh -= p.G;
-            ++qi;
+      for (it = -1;; ++it) {  // (-1: only the first segment's queries)
+        if (t > 0) {
+          ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (hf == 0 && q == 0 && lane == 0) mbar_arrive(&sm.seg_empty[(it - 1) % kSegments]);
+          if (!pend_idle) {
+            const float2 other = swap(pend.l, pend.nan);
+            if (!ok) break;
+            finish_row(pend, o_adr, pend.l + other.x, ((pend.nan | __float_as_uint(other.y)) >> hf) & 1u);
           }
+          if (!more) break;
         }
-        copy_commit();
-      };
-      auto post_q = [&](int i) {
-        copy_wait<0>();
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.q_full[i & 1][g]);
-      };
-      fetch_q(0);
-      post_q(0);
+        int u0 = 0, n = 0, row = 0, r0 = 0;
+        Span sp{};
+        if (it >= 0) {
+          const Segment& sg = segment(it);
+          if (!ok) break;
+          more = sg.more;
+          sp = sg.sp;
+          u0 = sg.u0, n = sg.n, r0 = sg.r0;
+        }
+        if (more) {
+          // the next segment's queries to their buffer (S of the segment before, its last
+          // reader, is done): each warp 16 rows, 4 rows an instruction
+          const Segment& sg = segment(it + 1);
+          if (!ok) break;
+          const int from = (hf * 4 + q) * 16;
+          const uint32_t dst = smem_u32(sm.q[(it + 1) & 1][g]) + from * 128;
+          const bf16* src = p.q + (long long)sg.b * p.q_batch + (long long)sg.h * p.G * HD + (lane & 7) * 8;
+          const int qrow = sg.r0 + g * BQ + from + (lane >> 3);
 #pragma unroll 1
-      for (bool more = true; ok; ++it) {
-        if (!more) break;
-        const Segment& sg = segment(it);
-        if (!ok) break;
-        more = sg.more;
-        // (the buffer's last reader, S of the segment before, is done)
-        if (more) fetch_q(it + 1);
-        if (!ok) break;
-        const Span sp = sg.sp;
-        const int u0 = sg.u0, n = sg.n, r0 = sg.r0;
-        const int row = r0 + g * BQ + q * 32 + lane, i = row / p.G;
-        const bool mine = row < rows && row < r0 + p.block;
-        const int pos = mine && i < sp.ql ? sp.pos(i, p.causal) : -1;
+          for (int k = 0; k < 16; k += 4) {
+            const int rr = (lane >> 3) + k, qi = (qrow + k) / p.G;
+            const bool in = qrow + k < rows;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             dst + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)),
+                         "l"(in ? src + (long long)qi * p.q_row + (qrow + k - qi * p.G) * HD : p.q), "r"(in ? 16 : 0)
+                         : "memory");
+          }
+          copy_commit();
+        }
+        row = r0 + g * BQ + q * 32 + lane;
+        const int i = row / p.G;
+        const bool none = i >= sp.ql;
+        const int pos = row < rows && !none ? sp.pos(i, p.causal) : -1;
         const bool idle = r0 + g * BQ + q * 32 >= rows;  // no row in this warp
         float m = -INFINITY, l = 0.f;
         uint32_t nan = 0;
 #pragma unroll 1
         for (int j = 0; j < n; ++j, ++t) {
-          ok = mbar_wait_bounded(&sm.s_full[g], (uint32_t)t & 1u, abort_flag);
+          const int tile = 2 * t + g, buf = tile % kBuffers;
+          ok = mbar_wait_bounded(&sm.s_full[buf], (uint32_t)(tile / kBuffers) & 1u, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          const int ua = 2 * (u0 + j), ka = sp.unit(ua), kb = sp.unit(ua + 1);  // pages
-          bool plain = ((ka >= sp.open && ka < sp.shut) || ka < sp.sink_open) &&
-                       ((kb >= sp.open && kb < sp.shut) || kb < sp.sink_open);
-          uint32_t vis[4] = {0u, 0u, 0u, 0u};  // keys that the row sees, set where not all are
-          {
-            const uint32_t f = smem_u32(&sm.flags[t % kFlags]);
-            const uint4 n0 = lds16(f), n1 = lds16(f + 16), ab = lds16(f + 32);
-            const uint32_t flagged = n0.x | n0.y | n0.z | n0.w | n1.x | n1.y | n1.z | n1.w;
-            plain = plain && (ab.x | ab.z) == 0u;
-            if (!plain || flagged != 0u) {
-              vis[0] = ab.x != 0u ? 0u : seen32(ka * kUnit, pos, p.window, p.sinks);
-              vis[1] = ab.x != 0u ? 0u : seen32(ka * kUnit + 32, pos, p.window, p.sinks);
-              vis[2] = ab.z != 0u ? 0u : seen32(kb * kUnit, pos, p.window, p.sinks);
-              vis[3] = ab.z != 0u ? 0u : seen32(kb * kUnit + 32, pos, p.window, p.sinks);
-              if (((n0.x & vis[0]) | (n0.y & vis[1]) | (n0.z & vis[2]) | (n0.w & vis[3])) != 0u) nan |= 1u;
-              if (((n1.x & vis[0]) | (n1.y & vis[1]) | (n1.z & vis[2]) | (n1.w & vis[3])) != 0u) nan |= 2u;
-            }
-          }
-          // The row goes by in quarters, the next one on its way from TMEM.  Exponentials
-          // are taken against the maximum so far while the unit's own is still being
-          // found; where that outgrows it by more than 2^8 (the first unit, then rarely)
-          // the quarters are gone through again.
-          uint32_t sa[2][32];
-          auto mask = [&](uint32_t* r, int qt) {
-            if (!plain) {
-              const uint32_t v = qt == 0 ? vis[0] : qt == 1 ? vis[1] : qt == 2 ? vis[2] : vis[3];
-#pragma unroll
-              for (int c = 0; c < 32; ++c) r[c] = (v >> c) & 1u ? r[c] : 0xFF800000u;
-            }
-          };
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          auto top = [&](const uint32_t* r) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
-            }
-          };
-          float rs[4] = {0.f, 0.f, 0.f, 0.f};
-          auto exps = [&](const uint32_t* r, int qt) {
-            const float mbase = m == -INFINITY ? 0.f : m;
-            uint32_t pk[16];
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              float x0, x1, e0, e1;
-              attn_tc::fma2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]), p.scale_log2, -mbase, x0, x1);
-              e0 = ex2(x0);
-              e1 = ex2(x1);
-              attn_tc::add2(rs[c & 2], rs[(c & 2) + 1], e0, e1);
-              pk[c >> 1] = pack_bf16x2(e0, e1);
-            }
-            tmem_put16(p_adr + qt * 16, pk);
-          };
-          if (!idle) tmem_start32(s_adr, sa[0]);
-          if (t > 0) {
-            // P_g and O_g were last used by P.V of unit t - 1
-            ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-          }
-          if (j == 0 && pending) {
-            if (q == 0 && lane == 0) mbar_arrive(&sm.seg_empty[(it - 1) % kSegments]);
-            finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_there, pend_whole, pend_slot);
-          }
           if (!idle) {
-            if (j == 0) {  // no maximum yet: the unit's own, first
-#pragma unroll 1
-              for (int qt = 0; qt < 4; qt += 2) {
-                tmem_wait32(sa[0]);
-                tmem_start32(s_adr + 32 * qt + 32, sa[1]);
-                mask(sa[0], qt);
-                top(sa[0]);
-                tmem_wait32(sa[1]);
-                tmem_start32(s_adr + (qt == 0 ? 64 : 0), sa[0]);
-                mask(sa[1], qt + 1);
-                top(sa[1]);
+            const uint32_t s_adr = s_adr0 + (uint32_t)(buf * kKeys);
+            uint32_t r[32];
+            tmem_start32(s_adr, r);
+            const int pg = sp.unit(2 * (u0 + j) + hf);
+            bool plain = (pg >= sp.open && pg < sp.shut) || pg < sp.sink_open;  // every row sees the page
+            uint32_t vis0 = 0u, vis1 = 0u;  // else: the keys that this one sees
+            {
+              const uint32_t f = smem_u32(&sm.flags[t % kFlags]);
+              const uint4 nn = lds16(f + 16 * hf), ab = lds16(f + 32);
+              const bool absent = (hf == 0 ? ab.x : ab.z) != 0u;
+              plain = plain && !absent;
+              if (!plain || (nn.x | nn.y | nn.z | nn.w) != 0u) {
+                vis0 = absent ? 0u : seen32(pg * kUnit, pos, p.window, p.sinks);
+                vis1 = absent ? 0u : seen32(pg * kUnit + 32, pos, p.window, p.sinks);
+                if (((nn.x & vis0) | (nn.y & vis1)) != 0u) nan |= 1u;
+                if (((nn.z & vis0) | (nn.w & vis1)) != 0u) nan |= 2u;
               }
-              m = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
             }
-            bool again = false;
-            float mx = m;
-#pragma unroll 1
-            for (int qt = 0; qt < 4; qt += 2) {
-              tmem_wait32(sa[0]);
-              tmem_start32(s_adr + 32 * qt + 32, sa[1]);
-              mask(sa[0], qt);
-              top(sa[0]);
-              exps(sa[0], qt);
-              tmem_wait32(sa[1]);
-              if (qt == 0) tmem_start32(s_adr + 64, sa[0]);
-              mask(sa[1], qt + 1);
-              top(sa[1]);
-              if (qt == 2) {
-                mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-                again = __any_sync(0xffffffffu, mx > m + kRescaleLog2);
-                if (!again) {
-                  tc_fence_before();
-                  mbar_arrive(&sm.s_free[g]);
-                }
+            auto mask = [&](uint32_t v) {
+              if (!plain) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) r[c] = (v >> c) & 1u ? r[c] : 0xFF800000u;
               }
-              exps(sa[1], qt + 1);
-            }
-            if (again) {
-              float alpha = 1.f;
-              if (mx > m + kRescaleLog2) {
-                alpha = ex2(m - mx);
+            };
+            // the row's maximum over the unit, from both threads
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto top = [&]() {
+#pragma unroll
+              for (int c = 0; c < 32; c += 8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  mx4[e] = max3(mx4[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
+              }
+            };
+            tmem_wait32(r);
+            mask(vis0);
+            top();
+            tmem_start32(s_adr + 32, r);
+            tmem_wait32(r);
+            mask(vis1);
+            top();
+            float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+            mx = fmaxf(mx, swap(mx, 0u).x);
+            if (!ok) break;
+            const bool grow = mx > m + kRescaleLog2;  // (from no maximum, always)
+            if (__any_sync(0xffffffffu, grow)) {
+              const float alpha = grow ? ex2(m - mx) : 1.f;
+              if (grow) {
                 m = mx;
                 l *= alpha;
               }
+              if (j > 0) {
+                ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < HD; c += 16) {
-                float o[16];
-                uint32_t u[16];
-                tmem_ld16(o_adr + c, o);
+                for (int c = 0; c < HD / 2; c += 16) {
+                  float o[16];
+                  uint32_t u[16];
+                  tmem_ld16(o_adr + c, o);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
-                attn_tc::tmem_st16(o_adr + c, u);
-              }
-#pragma unroll
-              for (int e = 0; e < 4; ++e) rs[e] = 0.f;
-              tmem_put_wait();
-#pragma unroll 1
-              for (int qt = 0; qt < 4; ++qt) {
-                tmem_start32(s_adr + 32 * qt, sa[0]);
-                tmem_wait32(sa[0]);
-                if (qt == 3) {
-                  tc_fence_before();
-                  mbar_arrive(&sm.s_free[g]);
+                  for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
+                  attn_tc::tmem_st16(o_adr + c, u);
                 }
-                mask(sa[0], qt);
-                exps(sa[0], qt);
+              }
+            }
+            // P = exp2(S - m), rounded to bf16, over the S of the same 32 keys
+            const float mbase = m == -INFINITY ? 0.f : m;
+            float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int qt = 1; qt >= 0; --qt) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 32; c += 2) {
+                float x0, x1;
+                attn_tc::fma2(__uint_as_float(r[c]), __uint_as_float(r[c + 1]), p.scale_log2, -mbase, x0, x1);
+                x0 = ex2(x0);
+                x1 = ex2(x1);
+                attn_tc::add2(rs[c & 2], rs[(c & 2) + 1], x0, x1);
+                pk[c >> 1] = pack_bf16x2(x0, x1);
+              }
+              tmem_put16(s_adr + 32 * qt, pk);
+              if (qt == 1) {
+                tmem_start32(s_adr, r);
+                tmem_wait32(r);
+                mask(vis0);
               }
             }
             tmem_put_wait();
-            const float sum = (rs[0] + rs[1]) + (rs[2] + rs[3]);
-            l += sum;
-          } else {
-            tc_fence_before();
-            mbar_arrive(&sm.s_free[g]);
+            l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+          }
+          if (j > 0) {  // P is announced in step with P.V, one phase at a time
+            ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
           }
           tc_fence_before();
           mbar_arrive(&sm.p_full[g]);
         }
         if (!ok) break;
-        if (more) post_q(it + 1);
-        pending = true;
-        pend_whole = sg.whole != 0;
-        pend_b = sg.b, pend_h = sg.h, pend_ql = sp.ql, pend_row = row, pend_there = mine, pend_m = m, pend_l = l, pend_nan = nan;
-        pend_slot = sg.slot + (row - r0);
-      }
-      if (ok && pending) {
-        ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) {
-          tc_fence_after();
-          finish_row(p, o_adr, pend_m, pend_l, pend_nan, pend_b, pend_h, pend_ql, pend_row, pend_there, pend_whole, pend_slot);
+        if (more) {
+          copy_wait<0>();
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.q_full[(it + 1) & 1][g]);
         }
+        if (it < 0) continue;
+        const Segment& sg = sm.seg[it % kSegments];
+        const long long slot = sg.slot + (row - r0);
+        const bool mine = row < rows, whole = sg.whole != 0;
+        pend_idle = idle;
+        pend.out = mine && whole ? p.o + (long long)sg.b * p.o_batch + (long long)i * p.o_row +
+                                       (long long)(sg.h * p.G + row - i * p.G) * HD + hf * (HD / 2)
+                                 : nullptr;
+        pend.part = mine && !whole ? p.part_o + slot * HD + hf * (HD / 2) : nullptr;
+        pend.ml = mine && !whole && hf == 0 ? reinterpret_cast<float2*>(p.part_ml + slot * 2) : nullptr;
+        pend.m = m, pend.l = l, pend.nan = nan, pend.none = none;
+      }
+      if (!ok) {  // release the row's other warp
+        if (lane == 0) *abort_flag = 1;
+        __syncwarp();
+        asm volatile("bar.arrive %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
       }
     }
     if (!ok && lane == 0) {
