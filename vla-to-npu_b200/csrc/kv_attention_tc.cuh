@@ -14,13 +14,12 @@
 //                three TMEM buffers in turn: it runs ahead of the softmax
 //   warp 2       P.V issuer in the same order: O_g += P V (P from TMEM, where its S was;
 //                V as the MN-major operand)
-//   warps 4..7   codes to bf16: each takes 32 keys of the unit, copies their codes
+//   warps 4..11  codes to bf16: each takes 16 keys of the unit, copies their codes
 //                and scales two units ahead (cp.async into a ring of its own) and
 //                writes code * scale, exact in bf16, into the swizzled K and V
-//                rings.  Against a bf16 cache this is what the kernel adds: about
-//                320 instructions per thread and unit beside the softmax's 2000
-//                issue slots.
-//   warps 8..23  softmax: two threads per row, each 64 of a unit's 128 keys (one
+//                rings.  This is what the kernel adds to one over a bf16 cache; four
+//                such warps took 2900 cycles a unit and held the others back.
+//   warps 12..27 softmax: two threads per row, each 64 of a unit's 128 keys (one
 //                page), which tell each other their maxima; they also bring the next
 //                segment's queries (cp.async).  Sixteen warps, because one warp's
 //                chain of TMEM loads, exponentials and packing, not any pipe, is what
@@ -42,12 +41,13 @@ namespace tc {
 constexpr int BQ = 128;
 constexpr int kRows = 2 * BQ;  // room for rows of an item (it has the whole query tokens that fit)
 constexpr int kKeys = 128;     // keys of a unit
-constexpr int kThreads = 768;
-constexpr int kLaunchRegs = 80;  // 65536 / 768, rounded down to a multiple of 8
-constexpr int kIssueRegs = 56;   // warps 0..3
-constexpr int kCodeRegs = 72;    // warps 4..7
-constexpr int kSoftRegs = 88;    // warps 8..23
-static_assert(kIssueRegs + kCodeRegs + 4 * kSoftRegs == 6 * kLaunchRegs, "register split must equal the launch total");
+constexpr int kCodeWarps = 8, kSoft0 = 4 + kCodeWarps;  // converting warps; the first softmax warp
+constexpr int kThreads = (kSoft0 + 16) * 32;
+constexpr int kLaunchRegs = 72;  // 65536 / 896, rounded down to a multiple of 8
+constexpr int kIssueRegs = 40;   // warps 0..3
+constexpr int kCodeRegs = 56;    // warps 4..11
+constexpr int kSoftRegs = 88;    // warps 12..27
+static_assert(kIssueRegs + 2 * kCodeRegs + 4 * kSoftRegs == 7 * kLaunchRegs, "register split must equal the launch total");
 constexpr int kRing = 3;    // K and V tiles
 constexpr int kFlags = 4;   // flag sets: a softmax thread reads set j before S(j+1) may be issued
 constexpr int TILE_BYTES = kKeys * HD * 2;
@@ -55,17 +55,17 @@ constexpr int kBuffers = 3;  // S and P of a tile (unit t, group g) in buffer (2
 constexpr uint32_t O_COL0 = kBuffers * kKeys;
 constexpr float kRescaleLog2 = 8.f;
 
-// What a converting warp copies: half a page.
+// What a converting warp copies: a tile of 16 keys.
 template <int BITS>
 struct Raw {
-  static constexpr int kCodes = kUnit / 2 * HD * BITS / 8;  // bytes of 32 keys' (or values') codes
-  static constexpr int kBytes = 2 * kCodes + 256;
+  static constexpr int kCodes = Block<BITS>::kTileCodes;  // of the keys, or of the values
+  static constexpr int kBytes = 2 * kCodes + 128;
   static constexpr int kStages = 3;
 };
 
 struct Flags {              // per page of a unit
-  uint32_t nan[2][4];       // keys whose value scale is NaN: [group 0: 32 keys, 32 keys, group 1: 32, 32]
-  uint32_t absent[2][2];    // per 32 keys: not there
+  uint16_t nan[2][2][4];    // [page][value group][tile]: keys whose scale is NaN
+  uint32_t absent[2][4];    // [page][tile]: not there (the same in a page's four)
 };
 
 // A CTA's share of an item, as warp 0 hands it to the other roles.
@@ -85,7 +85,7 @@ struct Smem {
   uint8_t q[2][2][TILE_BYTES];  // [buffer][tile]
   uint8_t k[kRing][TILE_BYTES];
   uint8_t v[kRing][TILE_BYTES];
-  uint8_t raw[4][Raw<BITS>::kStages][Raw<BITS>::kBytes];  // [warp]
+  uint8_t raw[kCodeWarps][Raw<BITS>::kStages][Raw<BITS>::kBytes];  // [warp]
   Flags flags[kFlags];
   Segment seg[kSegments];
   uint64_t seg_full[kSegments], seg_empty[kSegments];
@@ -127,29 +127,28 @@ __device__ __forceinline__ uint32_t seen32(int key0, int pos, int window, int si
   return m;
 }
 
-// 32 keys' codes to rows [r0, r0 + 32) of a K and a V tile.
+// A tile's codes to rows [r0, r0 + 16) of a K and a V tile.
 template <int BITS>
 __device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, int r0, int live, bool clean,
                                         uint32_t mask, int lane) {
   constexpr int C = Raw<BITS>::kCodes;
   const int g = lane >> 2, t = lane & 3;
-#pragma unroll 1
-  for (int tile = 0; tile < 2; ++tile) {
-    const uint32_t sc = raw + 2 * C + tile * 128;
+  {
+    const uint32_t sc = raw + 2 * C;
     // keys: tokens a and a + 2, 8 dims of either group
     const int a = 4 * (g >> 1) + (g & 1);
     uint4 d = lds16(sc + g * 16);
-    const int row = r0 + tile * 16 + a;
+    const int row = r0 + a;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {  // odd g the other way round: eight lanes then touch all banks
       const int grp = n ^ (g & 1);
       uint32_t c[2][4];
       if (BITS == 4) {
-        const uint4 w = lds16(raw + tile * 512 + lane * 16);
+        const uint4 w = lds16(raw + lane * 16);
         codes4(grp == 0 ? w.x : w.y, mask, c[0]);
         codes4(grp == 0 ? w.z : w.w, mask, c[1]);
       } else {
-        const uint4 w = lds16(raw + tile * 1024 + grp * 512 + lane * 16);
+        const uint4 w = lds16(raw + grp * 512 + lane * 16);
         codes8(w.x, mask, c[0]);
         codes8(w.y, mask, c[0] + 2);
         codes8(w.z, mask, c[1]);
@@ -169,17 +168,17 @@ __device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, 
     const uint32_t vs[4] = {sa.y, sb.y, sa.w, sb.w};
     uint4 w0, w1;
     if (BITS == 4) {
-      w0 = lds16(raw + C + tile * 512 + lane * 16);
+      w0 = lds16(raw + C + lane * 16);
     } else {
-      w0 = lds16(raw + C + tile * 1024 + lane * 16);
-      w1 = lds16(raw + C + tile * 1024 + 512 + lane * 16);
+      w0 = lds16(raw + C + lane * 16);
+      w1 = lds16(raw + C + 512 + lane * 16);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int rr = r0 + tile * 16 + 4 * q + r;
+      const int rr = r0 + 4 * q + r;
       uint32_t d0 = lo2(vs[r]), d1 = hi2(vs[r]);
       if (!clean) {  // past the end, or NaN (flagged)
-        const bool past = 4 * q + r + tile * 16 >= live;
+        const bool past = 4 * q + r >= live;
         if (past || (d0 & 0x7F80u) == 0x7F80u) d0 = 0u;
         if (past || (d1 & 0x7F80u) == 0x7F80u) d1 = 0u;
       }
@@ -283,9 +282,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.seg_empty[s], 2);
     }
     for (int s = 0; s < kRing; ++s) {
-      mbar_init(&sm.k_full[s], 4);
+      mbar_init(&sm.k_full[s], kCodeWarps);
       mbar_init(&sm.k_empty[s], 1);
-      mbar_init(&sm.v_full[s], 4);
+      mbar_init(&sm.v_full[s], kCodeWarps);
       mbar_init(&sm.v_empty[s], 1);
     }
     sm.abort = 0;
@@ -454,11 +453,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           t += n;
         }
       }
-    } else if (warp < 8) {
+    } else if (warp < kSoft0) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCodeRegs));
       // ---------------- codes to bf16 ----------------
       using Rw = Raw<BITS>;
-      const int w = warp - 4;  // keys [32 w, 32 w + 32) of a unit: half (w & 1) of page w >> 1
+      const int w = warp - 4;  // keys [16 w, 16 w + 16) of a unit: tile w % 4 of page w / 4
       const uint32_t raw = smem_u32(sm.raw[w]);
       // step c copies unit c and converts unit c - kStages + 1, each with a segment of its own
       int ci = 0, cu = 0, cn = 0, cb = 0, ch = 0, csink = 0, cfirst = 0, ccount = 0;
@@ -481,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           cmore = sg.more;
         }
         if (cn > 0) {
-          const int st = c % Rw::kStages, u = 2 * cu + (w >> 1);
+          const int st = c % Rw::kStages, u = 2 * cu + (w >> 2);
           bool have = false;
           if (u < ccount) {
             const int page = p.c.table[(long long)cb * p.c.table_ld + (u < csink ? u : cfirst + u - csink)];
@@ -489,14 +488,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (have) {
               const uint8_t* blk = p.c.pool + ((long long)page * heads + ch) * Block<BITS>::kBytes;
               const uint32_t dst = raw + st * Rw::kBytes + lane * 16;
-              const uint8_t* src = blk + (w & 1) * Rw::kCodes + lane * 16;
+              const uint8_t* src = blk + (w & 3) * Rw::kCodes + lane * 16;
 #pragma unroll
               for (int i = 0; i < Rw::kCodes / 512; ++i) {
                 copy16(dst + i * 512, src + i * 512);
                 copy16(dst + Rw::kCodes + i * 512, src + Block<BITS>::kValues + i * 512);
               }
-              if (lane < 16)
-                copy16(dst + 2 * Rw::kCodes, blk + Block<BITS>::kScales + (w & 1) * 256 + lane * 16);
+              if (lane < 8)
+                copy16(dst + 2 * Rw::kCodes, blk + Block<BITS>::kScales + (w & 3) * 128 + lane * 16);
             } else {
               vla_record_error(VLA_DERR_KV_RANGE);
             }
@@ -529,33 +528,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
           const uint32_t kt = smem_u32(sm.k[sr]), vt = smem_u32(sm.v[sr]), from = raw + st * Rw::kBytes;
-          const int u = 2 * (u0 + j) + (w >> 1), page = u < sink ? u : first + u - sink;
-          int live = 0;  // of the 32 keys, those inside the sequence
+          const int u = 2 * (u0 + j) + (w >> 2), page = u < sink ? u : first + u - sink;
+          int live = 0;  // of the 16 keys, those inside the sequence
           uint32_t n0 = 0u, n1 = 0u;
           if (have) {
-            live = min(32, len - (page * kUnit + (w & 1) * 32));
-            // key `lane`: tile lane / 16, token 4 q + b + 2 c at (2 q + b) * 16 + c * 8
-            const int tk = lane & 15;
+            live = min(16, len - (page * kUnit + (w & 3) * 16));
+            // key `lane`: token 4 q + b + 2 c at (2 q + b) * 16 + c * 8
             uint32_t s;
             asm volatile("ld.shared.u32 %0, [%1];"
                          : "=r"(s)
-                         : "r"(from + 2 * Rw::kCodes + (lane >> 4) * 128 + (2 * (tk >> 2) + (tk & 1)) * 16 +
-                               ((tk >> 1) & 1) * 8 + 4));
+                         : "r"(from + 2 * Rw::kCodes + (2 * ((lane & 15) >> 2) + (lane & 1)) * 16 + ((lane >> 1) & 1) * 8 + 4));
             n0 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F80u) == 0x7F80u);
             n1 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F800000u) == 0x7F800000u);
-            convert<BITS>(from, kt, vt, w * 32, live, live == 32 && (n0 | n1) == 0u, p.mask, lane);
+            convert<BITS>(from, kt, vt, w * 16, live, live == 16 && (n0 | n1) == 0u, p.mask, lane);
           } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              sts16(kt + w * 4096 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
-              sts16(vt + w * 4096 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
+            for (int i = 0; i < 4; ++i) {
+              sts16(kt + w * 2048 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
+              sts16(vt + w * 2048 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
             }
           }
           if (lane == 0) {
             Flags& f = sm.flags[t % kFlags];
-            f.nan[w >> 1][w & 1] = n0;
-            f.nan[w >> 1][2 + (w & 1)] = n1;
-            f.absent[w >> 1][w & 1] = have ? 0u : 1u;
+            f.nan[w >> 2][0][w & 3] = (uint16_t)n0;
+            f.nan[w >> 2][1][w & 3] = (uint16_t)n1;
+            f.absent[w >> 2][w & 3] = have ? 0u : 1u;
           }
           fence_async_smem();
           __syncwarp();
@@ -569,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
       // ---------------- softmax / output ----------------
-      const int g = (warp - 8) >> 3, hf = (warp >> 2) & 1, q = warp & 3;  // query tile, half of the keys, lane quarter
+      const int g = (warp - kSoft0) >> 3, hf = ((warp - kSoft0) >> 2) & 1, q = warp & 3;  // query tile, half of the keys, lane quarter
       const uint32_t lane_base = (uint32_t)(q * 32) << 16;
       const uint32_t s_adr0 = tmem + lane_base + (uint32_t)(hf * kUnit);
       const uint32_t o_adr = tmem + lane_base + O_COL0 + (uint32_t)(g * HD + hf * (HD / 2));
@@ -659,8 +656,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t vis0 = 0u, vis1 = 0u;  // else: the keys that this one sees
             {
               const uint32_t f = smem_u32(&sm.flags[t % kFlags]);
-              const uint4 nn = lds16(f + 16 * hf), ab = lds16(f + 32);
-              const bool absent = (hf == 0 ? ab.x : ab.z) != 0u;
+              const uint4 nn = lds16(f + 16 * hf);
+              const bool absent = lds16(f + 32 + 16 * hf).x != 0u;
               plain = plain && !absent;
               if (!plain || (nn.x | nn.y | nn.z | nn.w) != 0u) {
                 vis0 = absent ? 0u : seen32(pg * kUnit, pos, p.window, p.sinks);
