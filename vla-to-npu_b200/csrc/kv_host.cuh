@@ -60,12 +60,11 @@ static int append(const vla_kv_cache* c, const void* k, int64_t k_row, int64_t k
   VLA_TRY(check_rows(v, v_row, v_batch, width, "kv_append", "v"));
   AppendParams p{device_cache(c), (const bf16*)k, (const bf16*)v, (long long)k_row, (long long)v_row,
                  (long long)k_batch, (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4)};
-  const long long items = (long long)c->batch * p.quads * c->kv_heads;
-  VLA_CHECK_ARG((long long)p.quads * c->kv_heads < (1ll << 31) && (items + 7) / 8 < (1ll << 31),
-                "kv_append: too many rows");
+  const long long items = ((long long)p.quads + kQuads - 1) / kQuads * c->kv_heads;
+  VLA_CHECK_ARG(items < (1ll << 31) - 8, "kv_append: too many rows");
+  const dim3 grid((unsigned)((items + 7) / 8), c->batch < 65535 ? c->batch : 65535);
   prof_begin(st);
-  launch_k(c->bits == 4 ? append_kernel<4> : append_kernel<8>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, p,
-           items);
+  launch_k(c->bits == 4 ? append_kernel<4> : append_kernel<8>, grid, dim3(256), 0, st, p);
   prof_end(st, VLA_KIND_LAYOUT, 0.0,
            (double)c->batch * n * c->kv_heads * (4.0 * HD + (double)block_bytes(c->bits) / kPage));
   return launch_status("kv_append");
@@ -81,12 +80,11 @@ static int read(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, 
   VLA_TRY(check_rows(v, v_row, v_batch, width, "kv_read", "v"));
   ReadParams p{device_cache(c), (bf16*)k, (bf16*)v, (long long)k_row, (long long)v_row, (long long)k_batch,
                (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4)};
-  const long long items = (long long)c->batch * p.quads * c->kv_heads;
-  VLA_CHECK_ARG((long long)p.quads * c->kv_heads < (1ll << 31) && (items + 7) / 8 < (1ll << 31),
-                "kv_read: too many rows");
+  const long long items = ((long long)p.quads + kQuads - 1) / kQuads * c->kv_heads;
+  VLA_CHECK_ARG(items < (1ll << 31) - 8, "kv_read: too many rows");
+  const dim3 grid((unsigned)((items + 7) / 8), c->batch < 65535 ? c->batch : 65535);
   prof_begin(st);
-  launch_k(c->bits == 4 ? read_kernel<4> : read_kernel<8>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, p,
-           items);
+  launch_k(c->bits == 4 ? read_kernel<4> : read_kernel<8>, grid, dim3(256), 0, st, p);
   prof_end(st, VLA_KIND_LAYOUT, 0.0,
            (double)c->batch * n * c->kv_heads * (4.0 * HD + (double)block_bytes(c->bits) / kPage));
   return launch_status("kv_read");

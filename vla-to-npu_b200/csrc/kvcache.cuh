@@ -210,93 +210,100 @@ struct AppendParams {
   int quads;         // aligned groups of 4 positions that n tokens can touch
 };
 
-// Coordinates of one warp's item: (sequence, quad of 4 cache positions, kv head).
-struct Item {
-  int b, h, token, slot, off;  // token: index of the lane's token among the n; off: position inside the page
+// One warp takes kQuads neighbouring groups of 4 aligned cache positions of a
+// (sequence, kv head), lane = (token r, 8 dims w) of each.  blockIdx.x: (groups,
+// kv head), blockIdx.y: sequence.
+constexpr int kQuads = 2;
+
+struct Lane {
+  int token, slot, off;  // index of the lane's token among the n, page slot, position in the page
   bool live;
 };
-__device__ __forceinline__ Item item_of(long long w, int quads, int heads, int n, const int* start, const int* count,
-                                        int lane) {
-  Item it;
-  const int per = quads * heads;
-  it.b = (int)(w / per);
-  const int rem = (int)(w - (long long)it.b * per);
-  const int qd = rem / heads;
-  it.h = rem - qd * heads;
-  const int s = start != nullptr ? start[it.b] : 0;
-  const int valid = count != nullptr ? min(n, count[it.b]) : n;
-  const long long pos = (long long)((s >> 2) + qd) * 4 + (lane >> 3);
-  it.token = (int)(pos - s);
+__device__ __forceinline__ Lane lane_of(int start, int valid, int quad, int lane) {
+  Lane it;
+  const long long pos = ((long long)(start >> 2) + quad) * 4 + (lane >> 3);
+  it.token = (int)(pos - start);
   it.slot = (int)(pos / kPage);
   it.off = (int)(pos % kPage);
-  it.live = it.token >= 0 && it.token < valid;
-  if (s < 0) {
-    vla_record_error(VLA_DERR_KV_RANGE);
-    it.live = false;
-  }
+  it.live = start >= 0 && it.token >= 0 && it.token < valid;
   return it;
 }
 
-// One warp per (4 aligned cache positions, kv head): lane = (token r, 8 dims w).
-// It loads 16 bytes of K and of V per lane (each token's 128-byte row by 8
-// lanes), takes the scale over the 4 lanes of a group, and writes whole 128-byte
-// lines of codes (the order inside a tile keeps a quad's words together).
+// Each lane loads 16 bytes of K and of V per group (a token's 128-byte row by 8
+// lanes), takes the scale over the 4 lanes of a group of dims, and the warp
+// writes whole 128-byte lines of codes (the order inside a tile keeps a group's
+// words together).
 template <int BITS>
-__global__ void __launch_bounds__(256) append_kernel(AppendParams p, long long items) {
+__global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
   pdl_prologue();
   using B = Block<BITS>;
-  const long long warp = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (warp >= items) return;
   const int lane = threadIdx.x & 31, w = lane & 7;
-  const Item it = item_of(warp, p.quads, p.c.kv_heads, p.n, p.start, p.count, lane);
-  uint4 x[2];
-  x[0] = x[1] = make_uint4(0u, 0u, 0u, 0u);
-  uint8_t* blk = nullptr;
-  if (it.live) {
-    const long long col = (long long)it.h * HD + w * 8;
-    x[0] = ld_stream(p.k + (long long)it.b * p.k_batch + (long long)it.token * p.k_row + col);
-    x[1] = ld_stream(p.v + (long long)it.b * p.v_batch + (long long)it.token * p.v_row + col);
-    blk = block_of<BITS>(p.c, it.b, it.slot, it.h);
-  }
-  const int tile = it.off >> 4, q = (it.off >> 2) & 3, r = it.off & 3, t = w & 3, grp = w >> 2;
-  uint32_t dd[2];  // scales (bf16 bits)
+  const int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int q0 = item / p.c.kv_heads * kQuads, h = item % p.c.kv_heads;
+  if (q0 >= p.quads) return;
+  for (int b = blockIdx.y; b < p.c.batch; b += gridDim.y) {
+    const int s = p.start[b];
+    const int valid = p.count != nullptr ? min(p.n, p.count[b]) : p.n;
+    if (s < 0) vla_record_error(VLA_DERR_KV_RANGE);
+    Lane it[kQuads];
+    uint4 x[kQuads][2];
+    uint8_t* blk[kQuads];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {  // K, V
-    const uint32_t top = group_top(x[j]);
-    const float d = group_scale<BITS>((int)(short)(top & 0xFFFFu), (int)(short)(top >> 16));
-    dd[j] = __float_as_uint(d) >> 16;
-    float f[8];
-    unpack_bf16x8(x[j], f);
-    const float inv = 1.0f / d;
-    uint8_t* base = blk + (j == 0 ? 0 : B::kValues) + tile * B::kTileCodes;
-    if (BITS == 4) {
-      const uint32_t word = pack4(f, inv);
-      if (j == 0) {
-        if (blk) *reinterpret_cast<uint32_t*>(base + (2 * q + (r & 1)) * 64 + t * 16 + (r >> 1) * 8 + grp * 4) = word;
-      } else {
-        // a value word joins 4 dims of each group: swap halves with the other group's lane
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 4);
-        const uint32_t out = grp == 0 ? __byte_perm(word, other, 0x6240) : __byte_perm(other, word, 0x7351);
-        if (blk) *reinterpret_cast<uint32_t*>(base + q * 128 + (2 * t + grp) * 16 + r * 4) = out;
-      }
-    } else {
-      const uint32_t w0 = pack8(f, inv), w1 = pack8(f + 4, inv);
-      if (blk) {
-        base += grp * 512 + q * 128;
-        if (j == 0) {
-          *reinterpret_cast<uint2*>(base + (r & 1) * 64 + t * 16 + (r >> 1) * 8) = make_uint2(w0, w1);
-        } else {
-          *reinterpret_cast<uint32_t*>(base + (2 * t) * 16 + r * 4) = w0;
-          *reinterpret_cast<uint32_t*>(base + (2 * t + 1) * 16 + r * 4) = w1;
-        }
+    for (int u = 0; u < kQuads; ++u) {
+      it[u] = lane_of(s, valid, q0 + u, lane);
+      x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
+      blk[u] = nullptr;
+      if (it[u].live) {
+        const long long col = (long long)h * HD + w * 8;
+        x[u][0] = ld_stream(p.k + (long long)b * p.k_batch + (long long)it[u].token * p.k_row + col);
+        x[u][1] = ld_stream(p.v + (long long)b * p.v_batch + (long long)it[u].token * p.v_row + col);
+        blk[u] = block_of<BITS>(p.c, b, it[u].slot, h);
       }
     }
+#pragma unroll
+    for (int u = 0; u < kQuads; ++u) {
+      const int tile = it[u].off >> 4, q = (it[u].off >> 2) & 3, r = it[u].off & 3, t = w & 3, grp = w >> 2;
+      uint32_t dd[2];  // scales (bf16 bits)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {  // K, V
+        const uint32_t top = group_top(x[u][j]);
+        const float d = group_scale<BITS>((int)(short)(top & 0xFFFFu), (int)(short)(top >> 16));
+        dd[j] = __float_as_uint(d) >> 16;
+        float f[8];
+        unpack_bf16x8(x[u][j], f);
+        const float inv = 1.0f / d;
+        uint8_t* base = blk[u] + (j == 0 ? 0 : B::kValues) + tile * B::kTileCodes;
+        if (BITS == 4) {
+          const uint32_t word = pack4(f, inv);
+          if (j == 0) {
+            if (blk[u])
+              *reinterpret_cast<uint32_t*>(base + (2 * q + (r & 1)) * 64 + t * 16 + (r >> 1) * 8 + grp * 4) = word;
+          } else {
+            // a value word joins 4 dims of each group: swap halves with the other group's lane
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 4);
+            const uint32_t out = grp == 0 ? __byte_perm(word, other, 0x6240) : __byte_perm(other, word, 0x7351);
+            if (blk[u]) *reinterpret_cast<uint32_t*>(base + q * 128 + (2 * t + grp) * 16 + r * 4) = out;
+          }
+        } else {
+          const uint32_t w0 = pack8(f, inv), w1 = pack8(f + 4, inv);
+          if (blk[u]) {
+            base += grp * 512 + q * 128;
+            if (j == 0) {
+              *reinterpret_cast<uint2*>(base + (r & 1) * 64 + t * 16 + (r >> 1) * 8) = make_uint2(w0, w1);
+            } else {
+              *reinterpret_cast<uint32_t*>(base + (2 * t) * 16 + r * 4) = w0;
+              *reinterpret_cast<uint32_t*>(base + (2 * t + 1) * 16 + r * 4) = w1;
+            }
+          }
+        }
+      }
+      const uint32_t mine = dd[0] | dd[1] << 16;
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 4);
+      if (blk[u] && w == 0)
+        *reinterpret_cast<uint2*>(blk[u] + B::kScales + tile * 128 + (2 * q + (r & 1)) * 16 + (r >> 1) * 8) =
+            make_uint2(__byte_perm(mine, other, 0x5410), __byte_perm(mine, other, 0x7632));
+    }
   }
-  const uint32_t mine = dd[0] | dd[1] << 16;
-  const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 4);
-  if (blk && w == 0)
-    *reinterpret_cast<uint2*>(blk + B::kScales + tile * 128 + (2 * q + (r & 1)) * 16 + (r >> 1) * 8) =
-        make_uint2(__byte_perm(mine, other, 0x5410), __byte_perm(mine, other, 0x7632));
 }
 
 // ---------------------------------------------------------------------------
@@ -314,59 +321,77 @@ struct ReadParams {
 
 // The same mapping backwards; tokens past count are written as zeros.
 template <int BITS>
-__global__ void __launch_bounds__(256) read_kernel(ReadParams p, long long items) {
+__global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
   pdl_prologue();
   using B = Block<BITS>;
-  const long long warp = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (warp >= items) return;
-  const int lane = threadIdx.x & 31, w = lane & 7;
-  const Item it = item_of(warp, p.quads, p.c.kv_heads, p.n, p.start, p.count, lane);
-  const uint8_t* blk = it.live ? block_of<BITS>(p.c, it.b, it.slot, it.h) : nullptr;
-  const int tile = it.off >> 4, q = (it.off >> 2) & 3, r = it.off & 3, t = w & 3, grp = w >> 2;
-  uint32_t a[2][2] = {{0u, 0u}, {0u, 0u}};
-  uint2 sc = make_uint2(0u, 0u);
-  if (blk) {
-    const uint8_t* kb = blk + tile * B::kTileCodes;
-    const uint8_t* vb = kb + B::kValues;
-    if (BITS == 4) {
-      a[0][0] = ld_stream1(kb + (2 * q + (r & 1)) * 64 + t * 16 + (r >> 1) * 8 + grp * 4);
-      a[1][0] = ld_stream1(vb + q * 128 + (2 * t + grp) * 16 + r * 4);
-    } else {
-      kb += grp * 512 + q * 128;
-      vb += grp * 512 + q * 128;
-      const uint2 u = ld_stream2(kb + (r & 1) * 64 + t * 16 + (r >> 1) * 8);
-      a[0][0] = u.x;
-      a[0][1] = u.y;
-      a[1][0] = ld_stream1(vb + (2 * t) * 16 + r * 4);
-      a[1][1] = ld_stream1(vb + (2 * t + 1) * 16 + r * 4);
-    }
-    sc = ld_stream2(blk + B::kScales + tile * 128 + (2 * q + (r & 1)) * 16 + (r >> 1) * 8);
-  }
-  if (BITS == 4) {
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, a[1][0], 4);
-    // group 0's words hold bytes 0 and 2, group 1's bytes 1 and 3 of both value words
-    a[1][0] = grp == 0 ? __byte_perm(a[1][0], other, 0x6240) : __byte_perm(other, a[1][0], 0x7351);
-  }
-  if (it.token < 0 || it.token >= p.n) return;
-  const long long col = (long long)it.h * HD + w * 8;
+  const int lane = threadIdx.x & 31, w = lane & 7, t = w & 3, grp = w >> 2;
+  const int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int q0 = item / p.c.kv_heads * kQuads, h = item % p.c.kv_heads;
+  if (q0 >= p.quads) return;
+  for (int b = blockIdx.y; b < p.c.batch; b += gridDim.y) {
+    const int s = p.start != nullptr ? p.start[b] : 0;
+    const int valid = p.count != nullptr ? min(p.n, p.count[b]) : p.n;
+    if (s < 0) vla_record_error(VLA_DERR_KV_RANGE);
+    Lane it[kQuads];
+    const uint8_t* blk[kQuads];
+    uint32_t a[kQuads][2][2];
+    uint2 sc[kQuads];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t o[4] = {0u, 0u, 0u, 0u};
-    if (blk) {
-      const uint32_t s2 = j == 0 ? sc.x : sc.y;
-      const __nv_bfloat162 d = as_bf2(__byte_perm(s2, s2, grp == 0 ? 0x1010 : 0x3232));
+    for (int u = 0; u < kQuads; ++u) {
+      it[u] = lane_of(s, valid, q0 + u, lane);
+      blk[u] = it[u].live ? block_of<BITS>(p.c, b, it[u].slot, h) : nullptr;
+    }
+#pragma unroll
+    for (int u = 0; u < kQuads; ++u) {
+      const int tile = it[u].off >> 4, q = (it[u].off >> 2) & 3, r = it[u].off & 3;
+      a[u][0][0] = a[u][0][1] = a[u][1][0] = a[u][1][1] = 0u;
+      sc[u] = make_uint2(0u, 0u);
+      if (!blk[u]) continue;
+      const uint8_t* kb = blk[u] + tile * B::kTileCodes;
+      const uint8_t* vb = kb + B::kValues;
       if (BITS == 4) {
-        codes4(a[j][0], code_mask<4>(), o);
+        a[u][0][0] = ld_stream1(kb + (2 * q + (r & 1)) * 64 + t * 16 + (r >> 1) * 8 + grp * 4);
+        a[u][1][0] = ld_stream1(vb + q * 128 + (2 * t + grp) * 16 + r * 4);
       } else {
-        codes8(a[j][0], code_mask<8>(), o);
-        codes8(a[j][1], code_mask<8>(), o + 2);
+        kb += grp * 512 + q * 128;
+        vb += grp * 512 + q * 128;
+        const uint2 c = ld_stream2(kb + (r & 1) * 64 + t * 16 + (r >> 1) * 8);
+        a[u][0][0] = c.x;
+        a[u][0][1] = c.y;
+        a[u][1][0] = ld_stream1(vb + (2 * t) * 16 + r * 4);
+        a[u][1][1] = ld_stream1(vb + (2 * t + 1) * 16 + r * 4);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = as_u32(__hmul2(as_bf2(o[i]), d));
+      sc[u] = ld_stream2(blk[u] + B::kScales + tile * 128 + (2 * q + (r & 1)) * 16 + (r >> 1) * 8);
     }
-    bf16* dst = j == 0 ? p.k + (long long)it.b * p.k_batch + (long long)it.token * p.k_row + col
-                       : p.v + (long long)it.b * p.v_batch + (long long)it.token * p.v_row + col;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int u = 0; u < kQuads; ++u) {
+      if (BITS == 4) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, a[u][1][0], 4);
+        // group 0's words hold bytes 0 and 2, group 1's bytes 1 and 3 of both value words
+        a[u][1][0] = grp == 0 ? __byte_perm(a[u][1][0], other, 0x6240) : __byte_perm(other, a[u][1][0], 0x7351);
+      }
+      if (it[u].token < 0 || it[u].token >= p.n) continue;
+      const long long col = (long long)h * HD + w * 8;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t o[4] = {0u, 0u, 0u, 0u};
+        if (blk[u]) {
+          const uint32_t s2 = j == 0 ? sc[u].x : sc[u].y;
+          const __nv_bfloat162 d = as_bf2(__byte_perm(s2, s2, grp == 0 ? 0x1010 : 0x3232));
+          if (BITS == 4) {
+            codes4(a[u][j][0], code_mask<4>(), o);
+          } else {
+            codes8(a[u][j][0], code_mask<8>(), o);
+            codes8(a[u][j][1], code_mask<8>(), o + 2);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = as_u32(__hmul2(as_bf2(o[i]), d));
+        }
+        bf16* dst = j == 0 ? p.k + (long long)b * p.k_batch + (long long)it[u].token * p.k_row + col
+                           : p.v + (long long)b * p.v_batch + (long long)it[u].token * p.v_row + col;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
   }
 }
 

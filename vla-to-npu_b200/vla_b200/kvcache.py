@@ -77,8 +77,8 @@ class KVCache:
                              f"{pool.dtype} {tuple(pool.shape)}")
         if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError("table: need int32 [batch, max_pages] with unit column stride")
-        if table.device != pool.device:
-            raise ValueError(f"table is on {table.device}, the pool on {pool.device}")
+        if table.device != pool.device or not pool.is_cuda:
+            raise ValueError(f"table is on {table.device}, the pool on {pool.device}: need one CUDA device")
         self.pool, self.table = pool, table
         self.kv_heads, self.bits = kv_heads, bits
         self.batch, self.max_pages = table.shape
@@ -93,43 +93,58 @@ class KVCache:
             d.pages, d.max_pages, d.batch = pool.shape[1], self.max_pages, self.batch
             d.kv_heads, d.head_dim, d.bits = kv_heads, HEAD_DIM, bits
             self._desc.append((d, ctypes.byref(d)))
-        self._plans = {}
+        self._append, self._read = self._lib.vla_kv_append_bf16, self._lib.vla_kv_read_bf16
+        self._attend = self._lib.vla_kv_attention_bf16
+        self._dev = pool.get_device()
+        self._per_seq = torch.Size([self.batch])
+        self._strides, self._plans = {}, {}  # of shapes and strides: _rows; of sizes: workspace bytes
 
     # -- arguments ---------------------------------------------------------
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
-
+    # Calls of a few microseconds: what a shape, its strides and its type say is
+    # worked out once per combination, and the device is switched only if it has to be.
     def _index(self, t: Optional[torch.Tensor], name: str) -> Optional[int]:
         if t is None:
             return None
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != self.batch or t.device != self.device or \
+        if t.dtype is not torch.int32 or t.shape != self._per_seq or t.get_device() != self._dev or \
                 not t.is_contiguous():
             raise ValueError(f"{name}: need contiguous int32 [{self.batch}] on {self.device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
         return t.data_ptr()
 
-    def _rows(self, x: torch.Tensor, n: int, heads: int, name: str) -> Tuple[int, int, int]:
-        """(address, row stride, sequence stride) of [batch * n, heads * 64],
+    def _rows(self, x: torch.Tensor, n: int, heads: int, name: str) -> Tuple[int, int]:
+        """(row stride, sequence stride) of [batch * n, heads * 64],
         [batch, n, heads * 64] or [batch, n, heads, 64]."""
-        s, st = x.shape, x.stride()
-        d = len(s)
+        key = (x.shape, x.stride(), x.dtype, x.get_device(), n, heads)
+        got = self._strides.get(key)
+        if got is None:
+            if len(self._strides) >= 4096:  # callers with ever new lengths
+                self._strides.clear()
+            got = self._strides[key] = self._check_rows(x, n, heads, name)
+        return got
+
+    def _check_rows(self, x, n, heads, name):
+        s, st = tuple(x.shape), x.stride()
+        d, width = len(s), heads * HEAD_DIM
         if x.dtype != BF16 or x.device != self.device:
             raise ValueError(f"{name}: need bfloat16 on {self.device}, got {x.dtype} on {x.device}")
-        if d == 2 and s == (self.batch * n, heads * HEAD_DIM) and st[1] == 1:
+        if d == 2 and s == (self.batch * n, width) and st[1] == 1:
             row, batch = st[0], n * st[0]
-        elif d == 3 and s == (self.batch, n, heads * HEAD_DIM) and st[2] == 1:
+        elif d == 3 and s == (self.batch, n, width) and st[2] == 1:
             row, batch = st[1], st[0]
         elif d == 4 and s == (self.batch, n, heads, HEAD_DIM) and st[3] == 1 and (heads == 1 or st[2] == HEAD_DIM):
             row, batch = st[1], st[0]
         else:
-            raise ValueError(f"{name}: need [{self.batch * n}, {heads * HEAD_DIM}], [{self.batch}, {n}, "
-                             f"{heads * HEAD_DIM}] or [{self.batch}, {n}, {heads}, {HEAD_DIM}] with packed heads, got "
-                             f"{tuple(s)} strides {st}")
+            raise ValueError(f"{name}: need [{self.batch * n}, {width}], [{self.batch}, {n}, {width}] or "
+                             f"[{self.batch}, {n}, {heads}, {HEAD_DIM}] with packed heads, got {s} strides {st}")
         # a single row or sequence may have any stride
-        width = heads * HEAD_DIM
-        return x.data_ptr(), row if n > 1 or row >= width else width, batch if self.batch > 1 else 0
+        return row if n > 1 or row >= width else width, batch if self.batch > 1 else 0
 
-    def _check(self, rc: int) -> None:
+    def _call(self, fn, *args) -> None:
+        if torch._C._cuda_getDevice() == self._dev:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._dev))
+        else:
+            with torch.cuda.device(self._dev):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._dev))
         if rc != _lib.VLA_OK:
             raise _lib.VlaError(rc, _lib.last_error())
 
@@ -139,12 +154,10 @@ class KVCache:
         """Quantise ``n`` rows of K and V per sequence into tokens start[b] .. (the
         first count[b] of them, where given)."""
         h = self.kv_heads
-        kp, kr, kb = self._rows(k, n, h, "k")
-        vp, vr, vb = self._rows(v, n, h, "v")
-        with torch.cuda.device(self.device):
-            self._check(self._lib.vla_kv_append_bf16(self._desc[layer][1], kp, kr, kb, vp, vr, vb, n,
-                                                     self._index(start, "start"), self._index(count, "count"),
-                                                     self._stream()))
+        kr, kb = self._rows(k, n, h, "k")
+        vr, vb = self._rows(v, n, h, "v")
+        self._call(self._append, self._desc[layer][1], k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, n,
+                   self._index(start, "start"), self._index(count, "count"))
 
     def read(self, n: int, count: Optional[torch.Tensor] = None, start: Optional[torch.Tensor] = None, layer: int = 0,
              out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -152,13 +165,13 @@ class KVCache:
         [batch, n, kv_heads * 64]; rows from count[b] on are zeros."""
         h = self.kv_heads
         if out is None:
-            out = tuple(torch.empty(self.batch, n, h * HEAD_DIM, dtype=BF16, device=self.device) for _ in range(2))
-        kp, kr, kb = self._rows(out[0], n, h, "out k")
-        vp, vr, vb = self._rows(out[1], n, h, "out v")
-        with torch.cuda.device(self.device):
-            self._check(self._lib.vla_kv_read_bf16(self._desc[layer][1], kp, kr, kb, vp, vr, vb, n,
-                                                   self._index(start, "start"), self._index(count, "count"),
-                                                   self._stream()))
+            shape = (self.batch, n, h * HEAD_DIM)
+            out = torch.empty(shape, dtype=BF16, device=self.device), torch.empty(shape, dtype=BF16, device=self.device)
+        k, v = out
+        kr, kb = self._rows(k, n, h, "out k")
+        vr, vb = self._rows(v, n, h, "out v")
+        self._call(self._read, self._desc[layer][1], k.data_ptr(), kr, kb, v.data_ptr(), vr, vb, n,
+                   self._index(start, "start"), self._index(count, "count"))
         return out
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, causal: bool = True, window: int = 0, sinks: int = 0,
@@ -168,26 +181,31 @@ class KVCache:
         the first lens[b] tokens; the query tokens are the newest of them (causal)
         or read all of them.  ``window`` keeps the last keys up to each query,
         ``sinks`` the first ones as well."""
-        if q.dim() not in (3, 4) or q.shape[-1] % HEAD_DIM or q.dim() == 4 and q.shape[3] != HEAD_DIM:
-            raise ValueError(f"q: need [batch, Lq, heads, 64] or [batch, Lq, heads * 64], got {tuple(q.shape)}")
+        shape = q.shape
+        d = len(shape)
+        if d not in (3, 4) or shape[-1] % HEAD_DIM or d == 4 and shape[3] != HEAD_DIM:
+            raise ValueError(f"q: need [batch, Lq, heads, 64] or [batch, Lq, heads * 64], got {tuple(shape)}")
         if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31 and 0 <= max_len < 2 ** 31):
             raise ValueError(f"window={window}, sinks={sinks}, max_len={max_len}: need 0 .. 2^31 - 1")
-        n, heads = q.shape[1], q.shape[2] if q.dim() == 4 else q.shape[2] // HEAD_DIM
+        n, heads = shape[1], shape[2] if d == 4 else shape[2] // HEAD_DIM
         if out is None:
-            out = torch.empty(q.shape, dtype=BF16, device=self.device)
+            out = torch.empty(shape, dtype=BF16, device=self.device)
         a = _lib.KVAttentionArgs()
-        a.q, a.q_row, a.q_batch = self._rows(q, n, heads, "q")
-        a.o, a.o_row, a.o_batch = self._rows(out, n, heads, "out")
+        a.q, a.o = q.data_ptr(), out.data_ptr()
+        a.q_row, a.q_batch = self._rows(q, n, heads, "q")
+        a.o_row, a.o_batch = self._rows(out, n, heads, "out")
         a.lens, a.q_len = self._index(lens, "lens"), self._index(q_len, "q_len")
         a.Lq, a.Hq, a.causal, a.window, a.sinks, a.max_len, a.scale = n, heads, causal, window, sinks, max_len, scale
         desc, args = self._desc[layer][1], ctypes.byref(a)
-        with torch.cuda.device(self.device):
-            key = (n, heads, window, sinks, max_len)
-            need = self._plans.get(key)
-            if need is None:
+        key = (n, heads, window, sinks, max_len)
+        need = self._plans.get(key)
+        if need is None:
+            if len(self._plans) >= 4096:
+                self._plans.clear()
+            with torch.cuda.device(self._dev):
                 need = self._plans[key] = self._lib.vla_kv_attention_workspace(desc, args)
-            if need:
-                ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-                a.workspace, a.workspace_bytes = ws.data_ptr(), need
-            self._check(self._lib.vla_kv_attention_bf16(desc, args, self._stream()))
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        self._call(self._attend, desc, args)
         return out
