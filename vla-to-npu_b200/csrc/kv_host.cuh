@@ -43,6 +43,11 @@ static int check_rows(const void* x, int64_t row, int64_t batch, int64_t width, 
   return VLA_OK;
 }
 
+// Whether four groups of positions per warp leave a warp for each of the SMs' 64 places.
+static bool wide_rows(const vla_kv_cache* c, int quads) {
+  return (long long)c->batch * c->kv_heads * quads >= 4ll * 64 * device_info().num_sms;
+}
+
 #define VLA_TRY(expr)                \
   do {                               \
     const int _rc = (expr);          \
@@ -60,11 +65,14 @@ static int append(const vla_kv_cache* c, const void* k, int64_t k_row, int64_t k
   VLA_TRY(check_rows(v, v_row, v_batch, width, "kv_append", "v"));
   AppendParams p{device_cache(c), (const bf16*)k, (const bf16*)v, (long long)k_row, (long long)v_row,
                  (long long)k_batch, (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4)};
-  const long long items = ((long long)p.quads + kQuads - 1) / kQuads * c->kv_heads;
+  const bool many = wide_rows(c, p.quads);
+  const long long items = ((long long)p.quads + (many ? 3 : 0)) / (many ? 4 : 1) * c->kv_heads;
   VLA_CHECK_ARG(items < (1ll << 31) - 8, "kv_append: too many rows");
   const dim3 grid((unsigned)((items + 7) / 8), c->batch < 65535 ? c->batch : 65535);
   prof_begin(st);
-  launch_k(c->bits == 4 ? append_kernel<4> : append_kernel<8>, grid, dim3(256), 0, st, p);
+  launch_k(c->bits == 4 ? (many ? append_kernel<4, 4> : append_kernel<4, 1>)
+                        : (many ? append_kernel<8, 4> : append_kernel<8, 1>),
+           grid, dim3(256), 0, st, p);
   prof_end(st, VLA_KIND_LAYOUT, 0.0,
            (double)c->batch * n * c->kv_heads * (4.0 * HD + (double)block_bytes(c->bits) / kPage));
   return launch_status("kv_append");
@@ -79,12 +87,16 @@ static int read(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, 
   VLA_TRY(check_rows(k, k_row, k_batch, width, "kv_read", "k"));
   VLA_TRY(check_rows(v, v_row, v_batch, width, "kv_read", "v"));
   ReadParams p{device_cache(c), (bf16*)k, (bf16*)v, (long long)k_row, (long long)v_row, (long long)k_batch,
-               (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4)};
-  const long long items = ((long long)p.quads + kQuads - 1) / kQuads * c->kv_heads;
+               (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4),
+               c->bits == 4 ? code_mask<4>() : code_mask<8>()};
+  const bool many = wide_rows(c, p.quads);
+  const long long items = ((long long)p.quads + (many ? 3 : 0)) / (many ? 4 : 1) * c->kv_heads;
   VLA_CHECK_ARG(items < (1ll << 31) - 8, "kv_read: too many rows");
   const dim3 grid((unsigned)((items + 7) / 8), c->batch < 65535 ? c->batch : 65535);
   prof_begin(st);
-  launch_k(c->bits == 4 ? read_kernel<4> : read_kernel<8>, grid, dim3(256), 0, st, p);
+  launch_k(c->bits == 4 ? (many ? read_kernel<4, 4> : read_kernel<4, 1>)
+                        : (many ? read_kernel<8, 4> : read_kernel<8, 1>),
+           grid, dim3(256), 0, st, p);
   prof_end(st, VLA_KIND_LAYOUT, 0.0,
            (double)c->batch * n * c->kv_heads * (4.0 * HD + (double)block_bytes(c->bits) / kPage));
   return launch_status("kv_read");

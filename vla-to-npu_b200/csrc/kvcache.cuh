@@ -136,21 +136,29 @@ __device__ __forceinline__ float group_scale(int hp, int hn) {
   return top >= 0x7F00 ? __uint_as_float(0x7FC00000u) : d;  // 0x7F00 is 2^127
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Codes of 8 elements with the scale's reciprocal r.
-// 4 bits: x r differs from x / d by less than 2^-20, while a quotient of an
+// 4 bits: x r differs from x / d by less than 2^-20 (r is the hardware's reciprocal, off by
+// an ulp at most), while a quotient of an
 // 8-bit by a 5-bit significand that is no tie lies at least 2^-11 from every
 // half-integer within [-8.5, 8.5] (its distance is a multiple of 2^-5 / 62 when
 // it is near one at all).  The fused multiply-add onto 1.5 * 2^12 rounds to
 // multiples of 2^-11, which makes ties exact again and moves nothing else
 // across one; the second addition (1.5 * 2^23 + 8) rounds to integers, ties to
 // even, and leaves code + 8 in the low mantissa bits.
+// (The words are summed with those bits' constant part, which is taken off at the end.)
 __device__ __forceinline__ uint32_t pack4(const float* x, float r) {
   uint32_t w = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
+    const int shift = 4 * (e >> 1) + 16 * (e & 1);
     const float q = fminf(fmaf(x[e], r, 6144.f) - 6144.f, 7.f);
-    const uint32_t n = __float_as_uint(q + 12582920.f) & 15u;
-    w |= n << (4 * (e >> 1) + 16 * (e & 1));
+    w += (__float_as_uint(q + 12582920.f) - 0x4B400000u) << shift;
   }
   return w;
 }
@@ -210,10 +218,13 @@ struct AppendParams {
   int quads;         // aligned groups of 4 positions that n tokens can touch
 };
 
-// One warp takes kQuads neighbouring groups of 4 aligned cache positions of a
+// One warp takes QUADS neighbouring groups of 4 aligned cache positions of a
 // (sequence, kv head), lane = (token r, 8 dims w) of each.  blockIdx.x: (groups,
-// kv head), blockIdx.y: sequence.
-constexpr int kQuads = 2;
+// kv head), blockIdx.y: sequence.  Four groups keep four times the loads in flight
+// and share the coordinates' arithmetic, one is a shorter chain: reading 32
+// histories of up to 8001 tokens 64.5 us with four, 77.0 with one; a single
+// sequence's 113 tokens 2.8 and 1.7 us.  kv_host.cuh takes four where that still
+// fills the SMs' 64 warps.
 
 struct Lane {
   int token, slot, off;  // index of the lane's token among the n, page slot, position in the page
@@ -221,8 +232,8 @@ struct Lane {
 };
 __device__ __forceinline__ Lane lane_of(int start, int valid, int quad, int lane) {
   Lane it;
-  const long long pos = ((long long)(start >> 2) + quad) * 4 + (lane >> 3);
-  it.token = (int)(pos - start);
+  const uint32_t pos = (((uint32_t)start >> 2) + (uint32_t)quad) * 4u + (uint32_t)(lane >> 3);  // below 2^32
+  it.token = (int)(pos - (uint32_t)start);
   it.slot = (int)(pos / kPage);
   it.off = (int)(pos % kPage);
   it.live = start >= 0 && it.token >= 0 && it.token < valid;
@@ -233,35 +244,36 @@ __device__ __forceinline__ Lane lane_of(int start, int valid, int quad, int lane
 // lanes), takes the scale over the 4 lanes of a group of dims, and the warp
 // writes whole 128-byte lines of codes (the order inside a tile keeps a group's
 // words together).
-template <int BITS>
+template <int BITS, int QUADS>
 __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
   pdl_prologue();
   using B = Block<BITS>;
   const int lane = threadIdx.x & 31, w = lane & 7;
   const int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int q0 = item / p.c.kv_heads * kQuads, h = item % p.c.kv_heads;
+  const int q0 = item / p.c.kv_heads * QUADS, h = item % p.c.kv_heads;
   if (q0 >= p.quads) return;
   for (int b = blockIdx.y; b < p.c.batch; b += gridDim.y) {
     const int s = p.start[b];
     const int valid = p.count != nullptr ? min(p.n, p.count[b]) : p.n;
     if (s < 0) vla_record_error(VLA_DERR_KV_RANGE);
-    Lane it[kQuads];
-    uint4 x[kQuads][2];
-    uint8_t* blk[kQuads];
+    const bf16* kb = p.k + (long long)b * p.k_batch + h * HD + w * 8;
+    const bf16* vb = p.v + (long long)b * p.v_batch + h * HD + w * 8;
+    Lane it[QUADS];
+    uint4 x[QUADS][2];
+    uint8_t* blk[QUADS];
 #pragma unroll
-    for (int u = 0; u < kQuads; ++u) {
+    for (int u = 0; u < QUADS; ++u) {
       it[u] = lane_of(s, valid, q0 + u, lane);
       x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
       blk[u] = nullptr;
       if (it[u].live) {
-        const long long col = (long long)h * HD + w * 8;
-        x[u][0] = ld_stream(p.k + (long long)b * p.k_batch + (long long)it[u].token * p.k_row + col);
-        x[u][1] = ld_stream(p.v + (long long)b * p.v_batch + (long long)it[u].token * p.v_row + col);
+        x[u][0] = ld_stream(kb + (long long)it[u].token * p.k_row);
+        x[u][1] = ld_stream(vb + (long long)it[u].token * p.v_row);
         blk[u] = block_of<BITS>(p.c, b, it[u].slot, h);
       }
     }
 #pragma unroll
-    for (int u = 0; u < kQuads; ++u) {
+    for (int u = 0; u < QUADS; ++u) {
       const int tile = it[u].off >> 4, q = (it[u].off >> 2) & 3, r = it[u].off & 3, t = w & 3, grp = w >> 2;
       uint32_t dd[2];  // scales (bf16 bits)
 #pragma unroll
@@ -271,7 +283,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
         dd[j] = __float_as_uint(d) >> 16;
         float f[8];
         unpack_bf16x8(x[u][j], f);
-        const float inv = 1.0f / d;
+        const float inv = BITS == 4 ? rcp(d) : __uint_as_float(0x7F000000u - __float_as_uint(d));  // 2^-k of 2^k
         uint8_t* base = blk[u] + (j == 0 ? 0 : B::kValues) + tile * B::kTileCodes;
         if (BITS == 4) {
           const uint32_t word = pack4(f, inv);
@@ -317,32 +329,35 @@ struct ReadParams {
   const int* start;  // or null: 0
   const int* count;  // valid tokens from start on per sequence, or null: n
   int n, quads;
+  uint32_t mask;     // code_mask<BITS>()
 };
 
 // The same mapping backwards; tokens past count are written as zeros.
-template <int BITS>
+template <int BITS, int QUADS>
 __global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
   pdl_prologue();
   using B = Block<BITS>;
   const int lane = threadIdx.x & 31, w = lane & 7, t = w & 3, grp = w >> 2;
   const int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int q0 = item / p.c.kv_heads * kQuads, h = item % p.c.kv_heads;
+  const int q0 = item / p.c.kv_heads * QUADS, h = item % p.c.kv_heads;
   if (q0 >= p.quads) return;
   for (int b = blockIdx.y; b < p.c.batch; b += gridDim.y) {
     const int s = p.start != nullptr ? p.start[b] : 0;
     const int valid = p.count != nullptr ? min(p.n, p.count[b]) : p.n;
     if (s < 0) vla_record_error(VLA_DERR_KV_RANGE);
-    Lane it[kQuads];
-    const uint8_t* blk[kQuads];
-    uint32_t a[kQuads][2][2];
-    uint2 sc[kQuads];
+    bf16* kd = p.k + (long long)b * p.k_batch + h * HD + w * 8;
+    bf16* vd = p.v + (long long)b * p.v_batch + h * HD + w * 8;
+    Lane it[QUADS];
+    const uint8_t* blk[QUADS];
+    uint32_t a[QUADS][2][2];
+    uint2 sc[QUADS];
 #pragma unroll
-    for (int u = 0; u < kQuads; ++u) {
+    for (int u = 0; u < QUADS; ++u) {
       it[u] = lane_of(s, valid, q0 + u, lane);
       blk[u] = it[u].live ? block_of<BITS>(p.c, b, it[u].slot, h) : nullptr;
     }
 #pragma unroll
-    for (int u = 0; u < kQuads; ++u) {
+    for (int u = 0; u < QUADS; ++u) {
       const int tile = it[u].off >> 4, q = (it[u].off >> 2) & 3, r = it[u].off & 3;
       a[u][0][0] = a[u][0][1] = a[u][1][0] = a[u][1][1] = 0u;
       sc[u] = make_uint2(0u, 0u);
@@ -364,14 +379,13 @@ __global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
       sc[u] = ld_stream2(blk[u] + B::kScales + tile * 128 + (2 * q + (r & 1)) * 16 + (r >> 1) * 8);
     }
 #pragma unroll
-    for (int u = 0; u < kQuads; ++u) {
+    for (int u = 0; u < QUADS; ++u) {
       if (BITS == 4) {
         const uint32_t other = __shfl_xor_sync(0xffffffffu, a[u][1][0], 4);
         // group 0's words hold bytes 0 and 2, group 1's bytes 1 and 3 of both value words
         a[u][1][0] = grp == 0 ? __byte_perm(a[u][1][0], other, 0x6240) : __byte_perm(other, a[u][1][0], 0x7351);
       }
       if (it[u].token < 0 || it[u].token >= p.n) continue;
-      const long long col = (long long)h * HD + w * 8;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint32_t o[4] = {0u, 0u, 0u, 0u};
@@ -379,16 +393,15 @@ __global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
           const uint32_t s2 = j == 0 ? sc[u].x : sc[u].y;
           const __nv_bfloat162 d = as_bf2(__byte_perm(s2, s2, grp == 0 ? 0x1010 : 0x3232));
           if (BITS == 4) {
-            codes4(a[u][j][0], code_mask<4>(), o);
+            codes4(a[u][j][0], p.mask, o);
           } else {
-            codes8(a[u][j][0], code_mask<8>(), o);
-            codes8(a[u][j][1], code_mask<8>(), o + 2);
+            codes8(a[u][j][0], p.mask, o);
+            codes8(a[u][j][1], p.mask, o + 2);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] = as_u32(__hmul2(as_bf2(o[i]), d));
         }
-        bf16* dst = j == 0 ? p.k + (long long)b * p.k_batch + (long long)it[u].token * p.k_row + col
-                           : p.v + (long long)b * p.v_batch + (long long)it[u].token * p.v_row + col;
+        bf16* dst = j == 0 ? kd + (long long)it[u].token * p.k_row : vd + (long long)it[u].token * p.v_row;
         *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }

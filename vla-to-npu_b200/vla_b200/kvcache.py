@@ -165,8 +165,10 @@ class KVCache:
         [batch, n, kv_heads * 64]; rows from count[b] on are zeros."""
         h = self.kv_heads
         if out is None:
-            shape = (self.batch, n, h * HEAD_DIM)
-            out = torch.empty(shape, dtype=BF16, device=self.device), torch.empty(shape, dtype=BF16, device=self.device)
+            w = h * HEAD_DIM
+            shape, strides = (self.batch, n, w), (n * w, w, 1)
+            out = (torch.empty_strided(shape, strides, dtype=BF16, device=self.device),
+                   torch.empty_strided(shape, strides, dtype=BF16, device=self.device))
         k, v = out
         kr, kb = self._rows(k, n, h, "out k")
         vr, vb = self._rows(v, n, h, "out v")
@@ -189,7 +191,7 @@ class KVCache:
             raise ValueError(f"window={window}, sinks={sinks}, max_len={max_len}: need 0 .. 2^31 - 1")
         n, heads = shape[1], shape[2] if d == 4 else shape[2] // HEAD_DIM
         if out is None:
-            out = torch.empty(shape, dtype=BF16, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         a = _lib.KVAttentionArgs()
         a.q, a.o = q.data_ptr(), out.data_ptr()
         a.q_row, a.q_batch = self._rows(q, n, heads, "q")
@@ -205,7 +207,7 @@ class KVCache:
             with torch.cuda.device(self._dev):
                 need = self._plans[key] = self._lib.vla_kv_attention_workspace(desc, args)
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=self.device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         self._call(self._attend, desc, args)
         return out
