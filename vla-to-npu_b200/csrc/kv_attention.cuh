@@ -83,7 +83,7 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int r0, int 
 // D = A B + C with C and D apart, so that a start value need not be copied.
 __device__ __forceinline__ void mma16n8(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c0, float c1,
                                         float c2, float c3) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -94,7 +94,7 @@ __device__ __forceinline__ void mma16n8(float* d, const uint32_t* a, uint32_t b0
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -122,7 +122,7 @@ struct Ring {
   static constexpr int kVOff = kChunks * 512;
   static constexpr int kSOff = kVOff + kChunks * 640;
   static constexpr int kStage = kSOff + kTiles * 128;  // 5120 or 4864 bytes
-  static constexpr int kStages = BITS == 4 ? 2 : 3;
+  static constexpr int kStages = 2;
   static constexpr int kWarpBytes = kStage * kStages;
 };
 
