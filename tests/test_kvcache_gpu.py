@@ -396,3 +396,56 @@ def test_refusals(cuda):
         KVCache.wrap(torch.empty(1, 2, 100, dtype=torch.uint8, device="cuda"), i32([[0]]), 2, 4)
     with pytest.raises(ValueError, match="table"):
         KVCache.wrap(cache.pool, cache.table.long(), 2, 4)
+
+
+def test_many_rows_bad_pages_and_shared_queries(cuda):
+    """The kernel for many rows: a page that is not there, a page count that is odd, and
+    one sequence's queries for all (a zero stride)."""
+    from vla_b200 import _lib, device as dev
+    B, n, H = 3, 300, 2
+    cache, gen = make(B, n, H, 4)
+    k, v = rows_like(gen, B, n, H * 64), rows_like(gen, B, n, H * 64)
+    cache.append(k.cuda(), v.cuda(), i32([0] * B), n)
+    q = rows_like(gen, 1, 50, 6, 64).expand(B, 50, 6, 64)
+    hk, hv = (R.held(f64(x).reshape(B, n, H, 64), 4) for x in (k, v))
+    lens = [300, 193, 64]
+    got = cache.attend(q.cuda()[:1].expand(B, 50, 6, 64), i32(lens), causal=False)
+    want, mag, big = R.attend(f64(q), hk, hv, lens, causal=False)
+    assert np.all(np.abs(f64(got) - want) <= R.attend_bound(want, mag, big))
+    check_clean()
+    cache.table[0, 2] = 10 ** 6
+    got = cache.attend(q.cuda(), i32(lens), causal=False)
+    with pytest.raises(_lib.VlaError) as e:
+        dev.sync_check()
+    assert e.value.code == _lib.VLA_E_DEVICE_RANGE
+    keep = [j for j in range(n) if j // 64 != 2]
+    first, mag0, big0 = R.attend(f64(q)[:1], hk[:1, keep], hv[:1, keep], [len(keep)], causal=False)
+    want[0], mag[0], big[0] = first[0], mag0[0], big0[0]
+    assert np.all(np.abs(f64(got) - want) <= R.attend_bound(want, mag, big))
+
+
+@pytest.mark.parametrize("rows", [3, 60])
+def test_values_of_the_largest_size_do_not_leak_from_hidden_keys(cuda, rows):
+    """A key that a row does not see may hold values near bf16's end."""
+    cache, gen = make(1, 128, 1, 8)
+    k, v = rows_like(gen, 1, 100, 64), rows_like(gen, 1, 100, 64)
+    v[0, 99] = 1.6e38
+    cache.append(k.cuda(), v.cuda(), i32([0]), 100)
+    q = rows_like(gen, 1, rows, 3, 64)
+    got = cache.attend(q.cuda(), i32([100]))
+    hk, hv = (R.held(f64(x).reshape(1, 100, 1, 64), 8) for x in (k, v))
+    want, mag, big = R.attend(f64(q)[:, :-1], hk, hv, [99])
+    assert np.all(np.abs(f64(got)[:, :-1] - want) <= R.attend_bound(want, mag, big))
+
+
+def test_query_layouts_that_share_a_kernel_agree(cuda):
+    """The same row in a call of few rows and in one of many: within the two kernels' roundings."""
+    cache, gen = make(2, 500, 2, 4)
+    k, v = rows_like(gen, 2, 500, 128), rows_like(gen, 2, 500, 128)
+    cache.append(k.cuda(), v.cuda(), i32([0, 0]), 500)
+    q = rows_like(gen, 2, 40, 6, 64).cuda()
+    many = cache.attend(q, i32([500, 333]), window=100, sinks=5)
+    hv = R.held(f64(v).reshape(2, 500, 2, 64), 4)
+    for i in (0, 17, 39):
+        few = cache.attend(q[:, i:i + 1], i32([500 - 39 + i, 333 - 39 + i]), window=100, sinks=5)
+        assert np.all(np.abs(f64(few[:, 0]) - f64(many[:, i])) <= 2.0 ** -6 * np.abs(hv).max())
