@@ -449,3 +449,38 @@ def test_query_layouts_that_share_a_kernel_agree(cuda):
     for i in (0, 17, 39):
         few = cache.attend(q[:, i:i + 1], i32([500 - 39 + i, 333 - 39 + i]), window=100, sinks=5)
         assert np.all(np.abs(f64(few[:, 0]) - f64(many[:, i])) <= 2.0 ** -6 * np.abs(hv).max())
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_value_scales_of_very_different_size(cuda, rows):
+    """Values that grow and shrink by powers of two along the sequence, over bf16's range."""
+    n = 700
+    cache, gen = make(1, n, 1, 4)
+    k, v = rows_like(gen, 1, n, 64), rows_like(gen, 1, n, 64)
+    step = torch.randint(-12, 13, (1, n // 20, 1), generator=gen).float().repeat_interleave(20, 1)
+    for power in (-80.0, 0.0, 100.0):
+        vv = (v.float() * 2 ** (step + power)).to(BF16)
+        cache.append(k.cuda(), vv.cuda(), i32([0]), n)
+        q = (rows_like(gen, 1, rows, 3, 64) * 0.25).to(BF16)
+        hk, hv = (R.held(f64(x).reshape(1, n, 1, 64), 4) for x in (k, vv))
+        want, mag, big = R.attend(f64(q), hk, hv, [n])
+        err = np.abs(f64(cache.attend(q.cuda(), i32([n]))) - want)
+        assert np.all(err <= R.attend_bound(want, mag, big))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("rows", [1, 2, 8, 40])
+def test_a_nan_value_group_leaves_the_other_group(cuda, rows, bits):
+    """One token's second value group is NaN: the first 32 dims stay right, the rest is NaN where it is seen."""
+    n = 90
+    cache, gen = make(1, n, 1, bits)
+    k, v = rows_like(gen, 1, n, 64), rows_like(gen, 1, n, 64)
+    v[0, 20, 50] = float("inf")
+    cache.append(k.cuda(), v.cuda(), i32([0]), n)
+    q = rows_like(gen, 1, rows, 3, 64)
+    got = f64(cache.attend(q.cuda(), i32([n])))
+    hk, hv = (R.held(f64(x).reshape(1, n, 1, 64), bits) for x in (k, v))
+    want, mag, big = R.attend(f64(q), hk, np.nan_to_num(hv), [n])
+    bound = R.attend_bound(want, mag, big)
+    assert np.all(np.abs(got[..., :32] - want[..., :32]) <= bound[..., :32])
+    assert np.isnan(got[..., 32:]).all()

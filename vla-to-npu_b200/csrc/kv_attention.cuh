@@ -283,7 +283,12 @@ __device__ __forceinline__ void record_cut(const AttnParams& p, const Deal& d, i
 // with its own running maximum, sum and output, which are joined in shared memory
 // at the item's end.  A warp copies pages into its own ring ahead of its
 // computation (cp.async; no warp waits for another).
-template <int BITS, int NT>
+// TWICE: P^T goes through the product as the sum of two bf16 numbers, which takes its
+// rounding (2^-8 of each term, as much as the output's own) out of the result.
+// Used where the keys are few: there one of them often outweighs the rest, its
+// rounding does not average out, and the call costs its launch; over long caches
+// it would cost a tenth of the time.
+template <int BITS, int NT, bool TWICE>
 __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   pdl_prologue();
   constexpr int R = 8 * NT, kThreads = kWarps * 32;
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
       uint4 vc[BITS / 4];
 #pragma unroll
       for (int c = 0; c < BITS / 4; ++c) vc[c] = lds16(va + (i * (BITS / 4) + c) * 640);
-      uint32_t pt[NT][2][2];  // P^T operand [n-tile][group][key half]
+      uint32_t pt[NT][2][2], rest[NT][2][2];  // P^T operand [n-tile][group][key half], and what it lost
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint32_t d = k == 0 ? sc[i].y : sc[i].w;
@@ -540,9 +545,14 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
             if ((hidden[j] >> (4 * i + 2 * k)) & 1u) x0.x = x1.x = 0.f;
             if ((hidden[j] >> (4 * i + 2 * k)) & 2u) x0.y = x1.y = 0.f;
           }
-          // P^T rounded to bf16 with its value scales (2^-8 of each term, as bf16 values have)
-          pt[j][0][k] = transpose8(pack_bf16x2(x0.x, x0.y));
-          pt[j][1][k] = transpose8(pack_bf16x2(x1.x, x1.y));
+          // P^T with its value scales, rounded to bf16
+          const uint32_t h0 = pack_bf16x2(x0.x, x0.y), h1 = pack_bf16x2(x1.x, x1.y);
+          pt[j][0][k] = transpose8(h0);
+          pt[j][1][k] = transpose8(h1);
+          if (TWICE) {
+            rest[j][0][k] = transpose8(pack_bf16x2(x0.x - __uint_as_float(h0 << 16), x0.y - __uint_as_float(h0 & 0xFFFF0000u)));
+            rest[j][1][k] = transpose8(pack_bf16x2(x1.x - __uint_as_float(h1 << 16), x1.y - __uint_as_float(h1 & 0xFFFF0000u)));
+          }
         }
       }
 #pragma unroll
@@ -553,6 +563,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
         for (int j = 0; j < NT; ++j) {
           mma16n8(o[j][2 * grp], a[0], pt[j][grp][0], pt[j][grp][1]);
           mma16n8(o[j][2 * grp + 1], a[1], pt[j][grp][0], pt[j][grp][1]);
+          if (TWICE) {
+            mma16n8(o[j][2 * grp], a[0], rest[j][grp][0], rest[j][grp][1]);
+            mma16n8(o[j][2 * grp + 1], a[1], rest[j][grp][0], rest[j][grp][1]);
+          }
         }
       }
     }

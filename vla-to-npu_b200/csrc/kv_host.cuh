@@ -119,8 +119,9 @@ static int resident_ctas() {
   if (n.load(std::memory_order_relaxed) == 0) {
     constexpr int smem = attend_smem<BITS, NT>();
     int per = 0;
-    if (cudaFuncSetAttribute(attend_kernel<BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attend_kernel<BITS, NT>, kWarps * 32, smem) != cudaSuccess ||
+    if (cudaFuncSetAttribute(attend_kernel<BITS, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaFuncSetAttribute(attend_kernel<BITS, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attend_kernel<BITS, NT, false>, kWarps * 32, smem) != cudaSuccess ||
         per < 1) {
       cudaGetLastError();  // no device: sizes are still answered
       return 4 * device_info().num_sms;
@@ -174,7 +175,8 @@ static void launch_attend(const AttnParams& p, cudaStream_t st) {
   constexpr int smem = attend_smem<BITS, NT>();
   const int ctas = resident_ctas<BITS, NT>();
   const int items = p.c.batch * p.row_blocks * p.c.kv_heads;
-  launch_k(attend_kernel<BITS, NT>, dim3(p.split ? ctas : items), dim3(kWarps * 32), smem, st, p);
+  launch_k(p.split ? attend_kernel<BITS, NT, false> : attend_kernel<BITS, NT, true>, dim3(p.split ? ctas : items),
+           dim3(kWarps * 32), smem, st, p);
   if (p.split) {  // a CTA per row that is there
     const int slices = p.row_blocks > 1 ? 8 * NT : p.Lq * p.G;
     launch_k(join_kernel<8 * NT, kJoinWarps>, dim3(slices, ctas), dim3(kJoinWarps * 32), 0, st, p, p.scale_log2);
