@@ -25,6 +25,15 @@
 //                chain of TMEM loads, exponentials and packing, not any pipe, is what
 //                a unit waits for: with one thread per row (eight warps) 1024 rows over
 //                4 x 8192 keys took 190 us.
+// What bounds it.  A unit (256 rows x 128 keys) takes about 5000 SM cycles: the
+// exponentials alone are 2048 on the MUFU (49 % busy), the tensor pipe 1000; 69 %
+// of the issue slots are used, a third of them by waiting warps.  1024 rows over 4
+// caches of up to 8192 keys (15 / 5 heads, 4 bits): 170 us, 467 TFLOP/s.  One-unit
+// items pay the chain between segments (queries, first maximum, rows out): 50 rows
+// over each of 256 prefixes of up to 113 keys 66 us, 50 rows over 16 windows of 3729
+// keys 53 us.  Slower: an exponential token between the groups, exponentials partly
+// on the FMA pipe, polling with a sleep, queries by TMA (whole query tokens per
+// block leave a thirteenth block of 3072 rows).
 // A key that a row does not see must not reach it.  Its S is replaced by -inf;
 // its value has the probability 0, and 0 times a value must be 0: slots past a
 // sequence's length are written as zeros, and a value group whose scale is NaN
