@@ -484,3 +484,18 @@ def test_a_nan_value_group_leaves_the_other_group(cuda, rows, bits):
     bound = R.attend_bound(want, mag, big)
     assert np.all(np.abs(got[..., :32] - want[..., :32]) <= bound[..., :32])
     assert np.isnan(got[..., 32:]).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("room", [300, 700])
+@pytest.mark.parametrize("lens,q_len", [
+    ([0] * 37, None),
+    ([1 + 61 * i % 300 if i % 3 else 0 for i in range(130)] + [0] * 30, None),
+    ([0] * 50 + [113] * 40, [i % 18 for i in range(90)]),
+    ([300], [7]),
+])
+def test_many_rows_short_caches_with_empty_sequences(cuda, lens, q_len, room, bits):
+    """Items that are dealt out whole (room for few pages) or in units, empty ones at a
+    share's start, middle and end; rows that do not fill a block."""
+    run_case((17, 6, 3, lens, q_len, True, 0, 0), bits, room=room)
+    run_case((17, 6, 2, lens, q_len, False, 70, 3), bits, room=room)

@@ -46,12 +46,12 @@ struct AttnParams {
   long long q_row, q_batch, o_row, o_batch;
   const int* lens;   // keys of each sequence
   const int* q_len;  // valid query tokens per sequence, or null: Lq
-  int Lq, Hq, G;
+  int Lq, G;
   int causal, window, sinks;
   float scale_log2;
   uint32_t mask;     // code_mask<BITS>()
   int block, row_blocks;  // rows of a block, blocks per (sequence, kv head)
-  int split;         // 0: one CTA per (block of rows, kv head); 1: all units dealt out to the CTAs evenly
+  int split;         // 1: all units dealt out to the CTAs evenly; 0: items whole (here a CTA each)
   float* part_o;     // split: [CTA][2][8 NT][64]
   float* part_ml;    //        [CTA][2][8 NT][2]
   int4* cut;         //        [CTA]: the item that starts in this CTA and goes on in others

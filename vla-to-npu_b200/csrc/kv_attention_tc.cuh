@@ -8,7 +8,9 @@
 // first tokens and the window's).  The units of all items make one line that is
 // dealt out evenly to the persistent CTAs (kv_attention.cuh), so causal masks,
 // windows and uneven lengths leave no SM waiting; an item cut by a CTA's border
-// leaves fp32 sums that join_kernel adds.  Warp roles:
+// leaves fp32 sums that join_kernel adds.  Where an item has a few units at most
+// (split == 0), items are dealt out whole, which spares the counting of all
+// units before the first one and the second launch.  Warp roles:
 //   warp 0       the CTA's segments (shares of items), for the other roles
 //   warp 1       S issuer: S = Q_g K^T (128 x 128), unit by unit, group 0 then 1, into
 //                three TMEM buffers in turn: it runs ahead of the softmax
@@ -21,19 +23,24 @@
 //                such warps took 2900 cycles a unit and held the others back.
 //   warps 12..27 softmax: two threads per row, each 64 of a unit's 128 keys (one
 //                page), which tell each other their maxima; they also bring the next
-//                segment's queries (cp.async).  Sixteen warps, because one warp's
-//                chain of TMEM loads, exponentials and packing, not any pipe, is what
-//                a unit waits for: with one thread per row (eight warps) 1024 rows over
-//                4 x 8192 keys took 190 us.
+//                segment's queries (cp.async) and write a segment's rows out, after the
+//                next one's first scores, which do not need O: so the last P.V is not
+//                waited for by itself.  Sixteen warps, because one warp's chain of TMEM
+//                loads, exponentials and packing, not any pipe, is what a unit waits
+//                for: with one thread per row (eight warps) 1024 rows over 4 x 8192 keys
+//                took 190 us.
 // What bounds it.  A unit (256 rows x 128 keys) takes about 5000 SM cycles: the
 // exponentials alone are 2048 on the MUFU (49 % busy), the tensor pipe 1000; 69 %
 // of the issue slots are used, a third of them by waiting warps.  1024 rows over 4
-// caches of up to 8192 keys (15 / 5 heads, 4 bits): 170 us, 467 TFLOP/s.  One-unit
-// items pay the chain between segments (queries, first maximum, rows out): 50 rows
-// over each of 256 prefixes of up to 113 keys 66 us, 50 rows over 16 windows of 3729
-// keys 53 us.  Slower: an exponential token between the groups, exponentials partly
-// on the FMA pipe, polling with a sleep, queries by TMA (whole query tokens per
-// block leave a thirteenth block of 3072 rows).
+// caches of up to 8192 keys (15 / 5 heads, 4 bits): 172 us, 463 TFLOP/s.  One-unit
+// items are one chain of latencies each, about 8000 cycles (queries, scores, maximum,
+// exponentials, the last item's rows): 50 rows over each of 256 prefixes of up to 113
+// keys 54 us (66 with the rows out before the next scores and all units dealt out); 50
+// rows over 16 windows of 3729 keys 53 us.  Slower: an exponential token between the
+// groups, exponentials partly on the FMA pipe, polling with a sleep, queries by TMA
+// (whole query tokens per block leave a thirteenth block of 3072 rows) or by a warp of
+// their own (one warp's copies take 8000 cycles a segment), rows out by the converting
+// warps (61 us), the few-row kernel in blocks of 32 rows (177 us).
 // A key that a row does not see must not reach it.  Its S is replaced by -inf;
 // its value has the probability 0, and 0 times a value must be 0: slots past a
 // sequence's length are written as zeros, and a value group whose scale is NaN
@@ -48,7 +55,7 @@ namespace kv {
 namespace tc {
 
 constexpr int BQ = 128;
-constexpr int kRows = 2 * BQ;  // room for rows of an item (it has the whole query tokens that fit)
+constexpr int kRows = 2 * BQ;  // rows of an item
 constexpr int kKeys = 128;     // keys of a unit
 constexpr int kCodeWarps = 8, kSoft0 = 4 + kCodeWarps;  // converting warps; the first softmax warp
 constexpr int kThreads = (kSoft0 + 16) * 32;
@@ -77,16 +84,16 @@ struct Flags {              // per page of a unit
   uint32_t absent[2][4];    // [page][tile]: not there (the same in a page's four)
 };
 
-// A CTA's share of an item, as warp 0 hands it to the other roles.
+// A CTA's share of an item, as warp 0 hands it to the other roles; one without units ends
+// the CTA's work.
 struct Segment {
   Span sp;
   int b, h, r0;        // sequence, kv head, first row
   int u0, n;           // units [u0, u0 + n)
   int whole;           // ... are all of the item's
-  int more;            // another segment follows
   long long slot;      // of its part in the workspace, in rows
 };
-// Entries: one is written again when both softmax groups have seen its last P.V done.
+// Entries: one is written again when its rows are out.
 constexpr int kSegments = 8;
 
 template <int BITS>
@@ -98,12 +105,14 @@ struct Smem {
   Flags flags[kFlags];
   Segment seg[kSegments];
   uint64_t seg_full[kSegments], seg_empty[kSegments];
-  uint64_t q_full[2][2];  // [buffer][group]
+  uint64_t q_full[2];  // [buffer]
   uint64_t k_full[kRing], k_empty[kRing];
   uint64_t v_full[kRing], v_empty[kRing];
   uint64_t s_full[kBuffers], s_empty[kBuffers];  // per buffer
   uint64_t p_full[2], pv_done[2];                // per group
-  float2 swap[2][2][kRows];    // [turn][half of the keys]: what they tell each other
+  float swap[2][2][kRows];       // [turn][half of the keys]: maxima that a row's two threads tell each other
+  float sum[2][2][kRows], top[2][kRows];  // [segment's parity]: what a segment's rows are finished with
+  uint8_t nan[2][2][kRows];
   int scan[kThreads / 32];
   int group, left;
   uint32_t tmem_base;
@@ -205,37 +214,6 @@ __device__ __forceinline__ void convert(uint32_t raw, uint32_t kt, uint32_t vt, 
   }
 }
 
-// Where a thread's half of a finished row goes, and what it is divided by.
-struct Pending {
-  bf16* out;      // the output's 32 dims, or
-  float* part;    // the part slot's
-  float2* ml;     // ... and its maximum and sum, from one of the two threads
-  float m, l;
-  uint32_t nan;
-  bool none;      // the query token is not there: zeros
-};
-
-// 32 dims of a finished row of O_g.  The caller has waited for the last P.V, and l
-// and nan are the whole row's.
-__device__ __forceinline__ void finish_row(const Pending& d, uint32_t o_adr, float l, bool nan) {
-  const bool zero = d.none || (l == 0.f && !nan);
-  const float inv = 1.f / l;
-  float o[HD / 2];
-  tmem_ld32(o_adr, o);  // warp-collective: every lane loads
-  if (d.out != nullptr) {
-#pragma unroll
-    for (int c = 0; c < HD / 2; ++c) o[c] = zero ? 0.f : nan ? __uint_as_float(0x7FC00000u) : o[c] * inv;
-#pragma unroll
-    for (int c = 0; c < HD / 2; c += 8) *reinterpret_cast<uint4*>(d.out + c) = pack_bf16x8(o + c);
-  } else if (d.part != nullptr) {
-#pragma unroll
-    for (int c = 0; c < HD / 2; c += 4)
-      *reinterpret_cast<float4*>(d.part + c) =
-          nan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-    if (d.ml != nullptr) *d.ml = make_float2(d.m, l);
-  }
-}
-
 __device__ __forceinline__ void tmem_start32(uint32_t a, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -277,8 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.q_full[i][0], 8);
-      mbar_init(&sm.q_full[i][1], 8);
+      mbar_init(&sm.q_full[i], 16);
       mbar_init(&sm.p_full[i], 256);
       mbar_init(&sm.pv_done[i], 1);
     }
@@ -288,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < kSegments; ++s) {
       mbar_init(&sm.seg_full[s], 1);
-      mbar_init(&sm.seg_empty[s], 2);
+      mbar_init(&sm.seg_empty[s], 16);
     }
     for (int s = 0; s < kRing; ++s) {
       mbar_init(&sm.k_full[s], kCodeWarps);
@@ -306,10 +283,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sm.tmem_base;
   pdl_prologue();
 
-  // this CTA's share of the units
-  int left;
+  // this CTA's share of the units, or (short caches) of the items
+  int left, group0, at0;
   Deal d;
-  {
+  if (p.split) {
     const int chunk = (groups + kThreads - 1) / kThreads;
     const int ga = min(groups, (int)threadIdx.x * chunk), gb = min(groups, ga + chunk);
     int mine = 0, before;
@@ -330,20 +307,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm.left = at;
     }
     if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
-    // rows that see nothing belong to no unit
-#pragma unroll 1
-    for (int i = blockIdx.x; i < groups; i += gridDim.x) {
-      const int b = i / p.row_blocks, r0 = i % p.row_blocks * p.block;
-      if (units_of(p, i) > 0) continue;
-#pragma unroll 1
-      for (int x = threadIdx.x; x < heads * p.block * 8; x += kThreads) {
-        const int hh = x / (p.block * 8), row = r0 + (x >> 3) % p.block, qi = row / p.G;
-        if (row < rows)
-          *reinterpret_cast<uint4*>(p.o + (long long)b * p.o_batch + (long long)qi * p.o_row +
-                                    (long long)(hh * p.G + row - qi * p.G) * HD + (x & 7) * 8) = make_uint4(0, 0, 0, 0);
-      }
-    }
     __syncthreads();
+    group0 = sm.group;
+    at0 = sm.left;
+  } else {
+    d = deal_of(groups * heads, gridDim.x, 1);
+    const int f0 = d.begin(blockIdx.x);
+    left = (int)blockIdx.x < d.n ? d.begin(blockIdx.x + 1) - f0 : 0;
+    group0 = f0 / heads;
+    at0 = f0 - group0 * heads;
+  }
+  // rows that see nothing belong to no unit
+#pragma unroll 1
+  for (int i = blockIdx.x; i < groups; i += gridDim.x) {
+    const int b = i / p.row_blocks, r0 = i % p.row_blocks * p.block;
+    if (units_of(p, i) > 0) continue;
+#pragma unroll 1
+    for (int x = threadIdx.x; x < heads * p.block * 8; x += kThreads) {
+      const int hh = x / (p.block * 8), row = r0 + (x >> 3) % p.block, qi = row / p.G;
+      if (row < rows)
+        *reinterpret_cast<uint4*>(p.o + (long long)b * p.o_batch + (long long)qi * p.o_row +
+                                  (long long)(hh * p.G + row - qi * p.G) * HD + (x & 7) * 8) = make_uint4(0, 0, 0, 0);
+    }
   }
   if (left > 0) {
     bool ok = true;
@@ -357,60 +342,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
       if (warp == 0) {
         // ---------------- segments ----------------
-        int group = sm.group - 1, h = heads, u0 = 0, units = 0;
+        int group = group0 - 1, h = heads, u0 = 0, units = 0;
+        bool begin = true;
         Span sp;
 #pragma unroll 1
-        for (; ok && left > 0; ++it) {
-          if (h == heads) {  // the next group that has units
-#pragma unroll 1
-            do {
-              ++group;
-              sp = span_of(p, group / p.row_blocks, group % p.row_blocks * p.block, p.block);
-              units = (sp.count + 1) / 2;
-            } while (units == 0);
+        while (ok) {
+          if (left > 0 && h == heads) {
+            ++group;
+            sp = span_of(p, group / p.row_blocks, group % p.row_blocks * p.block, p.block);
+            units = (sp.count + 1) / 2;
             h = 0;
-            if (it == 0) {
-              h = sm.left / units;
-              u0 = sm.left - h * units;
+            if (begin) {
+              h = p.split ? at0 / units : at0;
+              u0 = p.split ? at0 - h * units : 0;
+              begin = false;
+            }
+            if (units == 0) {
+              left -= p.split ? 0 : heads - h;
+              h = heads;
+              continue;
             }
           }
-          const int n = min(units - u0, left);
-          left -= n;
+          const int n = left <= 0 ? 0 : p.split ? min(units - u0, left) : units;
+          left -= p.split ? n : 1;
           if (it >= kSegments)
             ok = mbar_wait_bounded(&sm.seg_empty[it % kSegments], ((it / kSegments) & 1) ^ 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (lane == 0) {
             Segment& sg = sm.seg[it % kSegments];
-            sg.sp = sp;
-            sg.b = group / p.row_blocks;
-            sg.h = h;
-            sg.r0 = group % p.row_blocks * p.block;
-            sg.u0 = u0;
             sg.n = n;
-            sg.whole = n == units;
-            sg.more = left > 0;
-            sg.slot = (2ll * blockIdx.x + (it > 0 ? 1 : 0)) * kRows;
+            if (n > 0) {
+              sg.sp = sp;
+              sg.b = group / p.row_blocks;
+              sg.h = h;
+              sg.r0 = group % p.row_blocks * p.block;
+              sg.u0 = u0;
+              sg.whole = n == units;
+              sg.slot = (2ll * blockIdx.x + (it > 0 ? 1 : 0)) * kRows;
+            }
             mbar_arrive(&sm.seg_full[it % kSegments]);
-            if (left == 0) record_cut(p, d, group, h, u0, u0 + n, units, it);
+            if (p.split && n > 0 && left == 0) record_cut(p, d, group, h, u0, u0 + n, units, it);
           }
+          if (n == 0) break;
           u0 = 0;
           ++h;
+          ++it;
         }
       } else if (warp == 1) {
         // ---------------- S issuer: group 0's tile, then group 1's ----------------
         constexpr uint32_t idesc_s = make_idesc_bf16(BQ, kKeys);
         int t = 0;
 #pragma unroll 1
-        for (bool more = true; more && ok; ++it) {
+        for (;; ++it) {
           const Segment& sg = segment(it);
-          if (!ok) break;
           const int n = sg.n, qb = it & 1;
-          more = sg.more;
+          if (!ok || n == 0) break;
 #pragma unroll 1
           for (int j = 0; ok && j < 2 * n; ++j) {
             const int tile = 2 * t + j, g = j & 1, buf = tile % kBuffers, sk = (tile >> 1) % kRing;
-            if (j < 2) ok = mbar_wait_bounded(&sm.q_full[qb][g], (it >> 1) & 1, abort_flag);
+            if (j == 0) ok = mbar_wait_bounded(&sm.q_full[qb], (it >> 1) & 1, abort_flag);
             if (ok) ok = mbar_wait_bounded(&sm.k_full[sk], ((tile >> 1) / kRing) & 1, abort_flag);
             if (ok) ok = mbar_wait_bounded(&sm.s_empty[buf], ((tile / kBuffers) & 1) ^ 1, abort_flag);
             if (!ok) break;
@@ -433,11 +424,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t idesc_pv = make_idesc_bf16(BQ, HD) | (1u << 16);  // B (V) is MN-major
         int t = 0;
 #pragma unroll 1
-        for (bool more = true; more && ok; ++it) {
-          const Segment& sg = segment(it);
-          if (!ok) break;
-          const int n = sg.n;
-          more = sg.more;
+        for (;; ++it) {
+          const int n = segment(it).n;
+          if (!ok || n == 0) break;
 #pragma unroll 1
           for (int j = 0; ok && j < 2 * n; ++j) {
             const int tile = 2 * t + j, g = j & 1, buf = tile % kBuffers, sv = (tile >> 1) % kRing;
@@ -471,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // step c copies unit c and converts unit c - kStages + 1, each with a segment of its own
       int ci = 0, cu = 0, cn = 0, cb = 0, ch = 0, csink = 0, cfirst = 0, ccount = 0;
       int u0 = 0, n = 0, j = 0, len = 0, sink = 0, first = 0;
-      bool cmore = true, more = true;
+      bool cmore = true;
       uint32_t there = 0;  // bit (stage): the page exists
 #pragma unroll 1
       for (int c = 0; ok; ++c) {
@@ -486,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           csink = sg.sp.sink;
           cfirst = sg.sp.first;
           ccount = sg.sp.count;
-          cmore = sg.more;
+          cmore = cn > 0;
         }
         if (cn > 0) {
           const int st = c % Rw::kStages, u = 2 * cu + (w >> 2);
@@ -517,15 +506,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = c - (Rw::kStages - 1);
         if (t < 0) continue;
         if (j == n) {
-          if (!more) break;
           const Segment& sg = segment(it++);
           if (!ok) break;
           n = sg.n;
+          if (n == 0) break;
           u0 = sg.u0;
           len = sg.sp.len;
           sink = sg.sp.sink;
           first = sg.sp.first;
-          more = sg.more;
           j = 0;
         }
         const int st = t % Rw::kStages, sr = t % kRing;
@@ -536,39 +524,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) ok = mbar_wait_bounded(&sm.v_empty[sr], ((t / kRing) & 1) ^ 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-          const uint32_t kt = smem_u32(sm.k[sr]), vt = smem_u32(sm.v[sr]), from = raw + st * Rw::kBytes;
-          const int u = 2 * (u0 + j) + (w >> 2), page = u < sink ? u : first + u - sink;
-          int live = 0;  // of the 16 keys, those inside the sequence
-          uint32_t n0 = 0u, n1 = 0u;
-          if (have) {
-            live = min(16, len - (page * kUnit + (w & 3) * 16));
-            // key `lane`: token 4 q + b + 2 c at (2 q + b) * 16 + c * 8
-            uint32_t s;
-            asm volatile("ld.shared.u32 %0, [%1];"
-                         : "=r"(s)
-                         : "r"(from + 2 * Rw::kCodes + (2 * ((lane & 15) >> 2) + (lane & 1)) * 16 + ((lane >> 1) & 1) * 8 + 4));
-            n0 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F80u) == 0x7F80u);
-            n1 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F800000u) == 0x7F800000u);
-            convert<BITS>(from, kt, vt, w * 16, live, live == 16 && (n0 | n1) == 0u, p.mask, lane);
-          } else {
+        const uint32_t kt = smem_u32(sm.k[sr]), vt = smem_u32(sm.v[sr]), from = raw + st * Rw::kBytes;
+        const int u = 2 * (u0 + j) + (w >> 2), page = u < sink ? u : first + u - sink;
+        int live = 0;  // of the 16 keys, those inside the sequence
+        uint32_t n0 = 0u, n1 = 0u;
+        if (have) {
+          live = min(16, len - (page * kUnit + (w & 3) * 16));
+          // key `lane`: token 4 q + b + 2 c at (2 q + b) * 16 + c * 8
+          uint32_t s;
+          asm volatile("ld.shared.u32 %0, [%1];"
+                       : "=r"(s)
+                       : "r"(from + 2 * Rw::kCodes + (2 * ((lane & 15) >> 2) + (lane & 1)) * 16 + ((lane >> 1) & 1) * 8 + 4));
+          n0 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F80u) == 0x7F80u);
+          n1 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F800000u) == 0x7F800000u);
+          convert<BITS>(from, kt, vt, w * 16, live, live == 16 && (n0 | n1) == 0u, p.mask, lane);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              sts16(kt + w * 2048 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
-              sts16(vt + w * 2048 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
-            }
+          for (int i = 0; i < 4; ++i) {
+            sts16(kt + w * 2048 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
+            sts16(vt + w * 2048 + i * 512 + lane * 16, 0u, 0u, 0u, 0u);
           }
-          if (lane == 0) {
-            Flags& f = sm.flags[t % kFlags];
-            f.nan[w >> 2][0][w & 3] = (uint16_t)n0;
-            f.nan[w >> 2][1][w & 3] = (uint16_t)n1;
-            f.absent[w >> 2][w & 3] = have ? 0u : 1u;
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&sm.k_full[sr]);
-            mbar_arrive(&sm.v_full[sr]);
-          }
+        }
+        if (lane == 0) {
+          Flags& f = sm.flags[t % kFlags];
+          f.nan[w >> 2][0][w & 3] = (uint16_t)n0;
+          f.nan[w >> 2][1][w & 3] = (uint16_t)n1;
+          f.absent[w >> 2][w & 3] = have ? 0u : 1u;
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.k_full[sr]);
+          mbar_arrive(&sm.v_full[sr]);
+        }
         ++j;
       }
       copy_wait<0>();
@@ -580,82 +568,110 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t s_adr0 = tmem + lane_base + (uint32_t)(hf * kUnit);
       const uint32_t o_adr = tmem + lane_base + O_COL0 + (uint32_t)(g * HD + hf * (HD / 2));
       int t = 0, turn = 0;
-      // Tells the row's other thread (v, bits), returns what it tells.  The two warps meet
+      // Tells the row's other thread v, returns what it tells.  The two warps meet
       // at a named barrier; one that gives up arrives there (below), so none is left waiting.
-      auto swap = [&](float v, uint32_t bits) {
-        const int at = g * BQ + q * 32 + lane;
-        sm.swap[turn & 1][hf][at] = make_float2(v, __uint_as_float(bits));
+      const int at = g * BQ + q * 32 + lane;
+      auto swap = [&](float v) {
+        sm.swap[turn & 1][hf][at] = v;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
-        float2 r;
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
-                     : "=f"(r.x), "=f"(r.y)
-                     : "r"(smem_u32(&sm.swap[turn & 1][hf ^ 1][at])));
+        float r;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(smem_u32(&sm.swap[turn & 1][hf ^ 1][at])));
         ++turn;
         if (*abort_flag) ok = false;  // (raised before the other warp gave up)
         return r;
       };
-      // what the last segment's rows are finished with, once its last P.V is done
-      Pending pend{};
-      bool pend_idle = true;
+      auto queries_there = [&]() {  // of the next segment
+        copy_wait<0>();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[(it + 1) & 1]);
+      };
+      // 32 dims of segment i's rows, whose last P.V is done
+      auto rows_out = [&](int i) {
+        const Segment& sg = sm.seg[i % kSegments];
+        const int row = sg.r0 + at, tok = row / p.G;
+        if (row - lane < rows) {
+          float o[HD / 2];
+          tmem_ld32(o_adr, o);  // warp-collective: every lane loads
+          const float l = sm.sum[i & 1][0][at] + sm.sum[i & 1][1][at];
+          const bool nan = ((sm.nan[i & 1][0][at] | sm.nan[i & 1][1][at]) >> hf) & 1u;
+          if (row < rows && sg.whole) {
+            const bool zero = tok >= sg.sp.ql || (l == 0.f && !nan);
+            const float inv = 1.f / l;
+#pragma unroll
+            for (int c = 0; c < HD / 2; ++c) o[c] = zero ? 0.f : nan ? __uint_as_float(0x7FC00000u) : o[c] * inv;
+            bf16* out = p.o + (long long)sg.b * p.o_batch + (long long)tok * p.o_row +
+                        (long long)(sg.h * p.G + row - tok * p.G) * HD + hf * (HD / 2);
+#pragma unroll
+            for (int c = 0; c < HD / 2; c += 8) *reinterpret_cast<uint4*>(out + c) = pack_bf16x8(o + c);
+          } else if (row < rows) {
+            const long long slot = sg.slot + at;
+            float* part = p.part_o + slot * HD + hf * (HD / 2);
+#pragma unroll
+            for (int c = 0; c < HD / 2; c += 4)
+              *reinterpret_cast<float4*>(part + c) =
+                  nan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            if (hf == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(sm.top[i & 1][at], l);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.seg_empty[i % kSegments]);
+      };
+      const int tokens4 = 4 / p.G, heads4 = 4 - tokens4 * p.G;
       bool more = true;
 #pragma unroll 1
       for (it = -1;; ++it) {  // (-1: only the first segment's queries)
-        if (t > 0) {
-          ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          if (hf == 0 && q == 0 && lane == 0) mbar_arrive(&sm.seg_empty[(it - 1) % kSegments]);
-          if (!pend_idle) {
-            const float2 other = swap(pend.l, pend.nan);
-            if (!ok) break;
-            finish_row(pend, o_adr, pend.l + other.x, ((pend.nan | __float_as_uint(other.y)) >> hf) & 1u);
-          }
-          if (!more) break;
-        }
-        int u0 = 0, n = 0, row = 0, r0 = 0;
-        Span sp{};
-        if (it >= 0) {
-          const Segment& sg = segment(it);
-          if (!ok) break;
-          more = sg.more;
-          sp = sg.sp;
-          u0 = sg.u0, n = sg.n, r0 = sg.r0;
-        }
         if (more) {
           // the next segment's queries to their buffer (S of the segment before, its last
           // reader, is done): each warp 16 rows, 4 rows an instruction
           const Segment& sg = segment(it + 1);
           if (!ok) break;
-          const int from = (hf * 4 + q) * 16;
-          const uint32_t dst = smem_u32(sm.q[(it + 1) & 1][g]) + from * 128;
-          const bf16* src = p.q + (long long)sg.b * p.q_batch + (long long)sg.h * p.G * HD + (lane & 7) * 8;
-          const int qrow = sg.r0 + g * BQ + from + (lane >> 3);
-#pragma unroll 1
-          for (int k = 0; k < 16; k += 4) {
-            const int rr = (lane >> 3) + k, qi = (qrow + k) / p.G;
-            const bool in = qrow + k < rows;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                             dst + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)),
-                         "l"(in ? src + (long long)qi * p.q_row + (qrow + k - qi * p.G) * HD : p.q), "r"(in ? 16 : 0)
-                         : "memory");
+          more = sg.n > 0;
+          if (more) {
+            const int from = (hf * 4 + q) * 16 + (lane >> 3), qrow = sg.r0 + g * BQ + from;
+            const uint32_t dst = smem_u32(sm.q[(it + 1) & 1][g]) + from * 128;
+            int qi = qrow / p.G, head = qrow - qi * p.G;
+            const bf16* src = p.q + (long long)sg.b * p.q_batch + (long long)sg.h * p.G * HD + (lane & 7) * 8;
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+              const bool in = qrow + k < rows;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                               dst + k * 128 + (((lane & 7) ^ ((from + k) & 7)) << 4)),
+                           "l"(in ? src + (long long)qi * p.q_row + head * HD : p.q), "r"(in ? 16 : 0)
+                           : "memory");
+              qi += tokens4;
+              head += heads4;
+              if (head >= p.G) {
+                head -= p.G;
+                ++qi;
+              }
+            }
+            copy_commit();
           }
-          copy_commit();
         }
-        row = r0 + g * BQ + q * 32 + lane;
+        if (it < 0) {
+          if (!more) break;
+          queries_there();
+          continue;
+        }
+        const Segment& sg = sm.seg[it % kSegments];
+        const Span sp = sg.sp;
+        const int u0 = sg.u0, n = sg.n, r0 = sg.r0, row = r0 + at;
         const int i = row / p.G;
         const bool none = i >= sp.ql;
         const int pos = row < rows && !none ? sp.pos(i, p.causal) : -1;
-        const bool idle = r0 + g * BQ + q * 32 >= rows;  // no row in this warp
+        const bool idle = n == 0 || row - lane >= rows;  // no row in this warp
         float m = -INFINITY, l = 0.f;
         uint32_t nan = 0;
 #pragma unroll 1
-        for (int j = 0; j < n; ++j, ++t) {
+        for (int j = 0; j < n || j == 0; ++j, ++t) {
           const int tile = 2 * t + g, buf = tile % kBuffers;
-          ok = mbar_wait_bounded(&sm.s_full[buf], (uint32_t)(tile / kBuffers) & 1u, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
+          if (n > 0) {
+            ok = mbar_wait_bounded(&sm.s_full[buf], (uint32_t)(tile / kBuffers) & 1u, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+          }
           if (!idle) {
             const uint32_t s_adr = s_adr0 + (uint32_t)(buf * kKeys);
             uint32_t r[32];
@@ -699,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mask(vis1);
             top();
             float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-            mx = fmaxf(mx, swap(mx, 0u).x);
+            mx = fmaxf(mx, swap(mx));
             if (!ok) break;
             const bool grow = mx > m + kRescaleLog2;  // (from no maximum, always)
             if (__any_sync(0xffffffffu, grow)) {
@@ -749,32 +765,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_put_wait();
             l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
           }
-          if (j > 0) {  // P is announced in step with P.V, one phase at a time
+          if (t > 0) {  // P is announced in step with P.V, one phase at a time
             ok = mbar_wait_bounded(&sm.pv_done[g], (uint32_t)(t - 1) & 1u, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            if (j == 0) {
+              // the last segment's O, before this one's: its rows leave while their P.V and this
+              // segment's scores would only have been waited for
+              if (idle) swap(0.f);  // (else the maxima's: the other thread's sum is there)
+              if (!ok) break;
+              tc_fence_after();
+              int last = it - 1;
+              asm volatile("" : "+r"(last));  // keeps what rows_out derives from it out of the loop's registers
+              rows_out(last);
+            }
           }
+          if (n == 0) break;
           tc_fence_before();
           mbar_arrive(&sm.p_full[g]);
         }
-        if (!ok) break;
-        if (more) {
-          copy_wait<0>();
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.q_full[(it + 1) & 1][g]);
-        }
-        if (it < 0) continue;
-        const Segment& sg = sm.seg[it % kSegments];
-        const long long slot = sg.slot + (row - r0);
-        const bool mine = row < rows, whole = sg.whole != 0;
-        pend_idle = idle;
-        pend.out = mine && whole ? p.o + (long long)sg.b * p.o_batch + (long long)i * p.o_row +
-                                       (long long)(sg.h * p.G + row - i * p.G) * HD + hf * (HD / 2)
-                                 : nullptr;
-        pend.part = mine && !whole ? p.part_o + slot * HD + hf * (HD / 2) : nullptr;
-        pend.ml = mine && !whole && hf == 0 ? reinterpret_cast<float2*>(p.part_ml + slot * 2) : nullptr;
-        pend.m = m, pend.l = l, pend.nan = nan, pend.none = none;
+        if (!ok || n == 0) break;
+        if (more) queries_there();
+        sm.sum[it & 1][hf][at] = l;
+        sm.nan[it & 1][hf][at] = (uint8_t)nan;
+        if (hf == 0) sm.top[it & 1][at] = m;
       }
       if (!ok) {  // release the row's other warp
         if (lane == 0) *abort_flag = 1;

@@ -154,8 +154,8 @@ static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a,
   out->block = block;
   out->slots = out->nt > 0 ? block : tc::kRows;
   out->row_blocks = (int)blocks;
-  out->split = out->nt == 0 || keys > 8 * kUnit;
-  const size_t ctas = out->nt == 0 ? device_info().num_sms : out->split ? resident_ctas(c->bits, out->nt) : 0;
+  out->split = keys > 8 * kUnit;
+  const size_t ctas = !out->split ? 0 : out->nt == 0 ? device_info().num_sms : resident_ctas(c->bits, out->nt);
   out->workspace = ctas * (2 * out->slots * (HD + 2) * sizeof(float) + sizeof(int4));
   return VLA_OK;
 }
@@ -201,8 +201,10 @@ static int launch_tc(const AttnParams& p, cudaStream_t st) {
   }
   const int ctas = device_info().num_sms;
   launch_k(tc::attend_kernel<BITS>, dim3(ctas), dim3(tc::kThreads), smem, st, p);
-  const int slices = ((p.row_blocks > 1 ? p.block : p.Lq * p.G) + kJoinWarps - 1) / kJoinWarps;
-  launch_k(join_kernel<tc::kRows, 1>, dim3(slices, ctas), dim3(kJoinWarps * 32), 0, st, p, 1.f);
+  if (p.split) {
+    const int slices = ((p.row_blocks > 1 ? p.block : p.Lq * p.G) + kJoinWarps - 1) / kJoinWarps;
+    launch_k(join_kernel<tc::kRows, 1>, dim3(slices, ctas), dim3(kJoinWarps * 32), 0, st, p, 1.f);
+  }
   return VLA_OK;
 }
 
@@ -237,7 +239,6 @@ static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cuda
   p.lens = a->lens;
   p.q_len = a->q_len;
   p.Lq = a->Lq;
-  p.Hq = a->Hq;
   p.G = a->Hq / c->kv_heads;
   p.causal = a->causal != 0;
   // a window as long as the cache hides nothing, and first tokens mean nothing without one
