@@ -149,18 +149,22 @@ __device__ __forceinline__ float rcp(float x) {
 // half-integer within [-8.5, 8.5] (its distance is a multiple of 2^-5 / 62 when
 // it is near one at all).  The fused multiply-add onto 1.5 * 2^12 rounds to
 // multiples of 2^-11, which makes ties exact again and moves nothing else
-// across one; the second addition (1.5 * 2^23 + 8) rounds to integers, ties to
-// even, and leaves code + 8 in the low mantissa bits.
-// (The words are summed with those bits' constant part, which is taken off at the end.)
+// across one; the addition of 1.5 * 2^23 rounds to integers, ties to even.  The
+// codes + 8 stay floats until a half-word is summed (base 16, below 2^16: exact), two
+// half-words per instruction, which spares the integer pipe the shifts.
 __device__ __forceinline__ uint32_t pack4(const float* x, float r) {
-  uint32_t w = 0;
+  auto both = [](float v) { return make_float2(v, v); };
+  float2 w = both(0.f);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int shift = 4 * (e >> 1) + 16 * (e & 1);
-    const float q = fminf(fmaf(x[e], r, 6144.f) - 6144.f, 7.f);
-    w += (__float_as_uint(q + 12582920.f) - 0x4B400000u) << shift;
+  for (int i = 3; i >= 0; --i) {
+    float2 q = __fadd2_rn(__ffma2_rn(make_float2(x[2 * i], x[2 * i + 1]), both(r), both(6144.f)), both(-6144.f));
+    q.x = fminf(q.x, 7.f);
+    q.y = fminf(q.y, 7.f);
+    q = __fadd2_rn(__fadd2_rn(q, both(12582912.f)), both(-12582904.f));
+    w = i == 3 ? q : __ffma2_rn(w, both(16.f), q);
   }
-  return w;
+  w = __fadd2_rn(w, both(8388608.f));  // 2^23: the sum in the low mantissa bits
+  return __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x5410);
 }
 // 8 bits: d is a power of two, so x r is exact and one rounding does it.
 __device__ __forceinline__ uint32_t pack8(const float* x, float r) {
