@@ -45,7 +45,7 @@ static int check_rows(const void* x, int64_t row, int64_t batch, int64_t width, 
 
 // Whether four groups of positions per warp leave a warp for each of the SMs' 64 places.
 static bool wide_rows(const vla_kv_cache* c, int quads) {
-  return (long long)c->batch * c->kv_heads * quads >= 4ll * 64 * device_info().num_sms;
+  return (long long)c->batch * c->kv_heads * ((quads + 3ll) / 4) >= 64ll * device_info().num_sms;
 }
 
 #define VLA_TRY(expr)                \

@@ -248,7 +248,7 @@ __device__ __forceinline__ Lane lane_of(int start, int valid, int quad, int lane
 // lanes), takes the scale over the 4 lanes of a group of dims, and the warp
 // writes whole 128-byte lines of codes (the order inside a tile keeps a group's
 // words together).  Bound by its instructions at this size: 256 sequences of 113
-// rows (15 / 5 heads, 4 bits), written and read back, take 28 us of which the bytes
+// rows (15 / 5 heads, 4 bits), written and read back, take 27 us of which the bytes
 // need 15; 16 x 4001 rows in 8 bits 50 of 39 us.  Reading alone comes to 0.92 of the
 // measured copy rate (32 x 8001 tokens, 65 us).
 template <int BITS, int QUADS>
