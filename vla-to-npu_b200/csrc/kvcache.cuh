@@ -248,11 +248,13 @@ __device__ __forceinline__ Lane lane_of(int start, int valid, int quad, int lane
 // lanes), takes the scale over the 4 lanes of a group of dims, and the warp
 // writes whole 128-byte lines of codes (the order inside a tile keeps a group's
 // words together).  Bound by its instructions at this size: 256 sequences of 113
-// rows (15 / 5 heads, 4 bits), written and read back, take 27 us of which the bytes
-// need 15; 16 x 4001 rows in 8 bits 50 of 39 us.  Reading alone comes to 0.92 of the
-// measured copy rate (32 x 8001 tokens, 65 us).
+// rows (15 / 5 heads, 4 bits), written and read back, take 26.5 us of which the bytes
+// need 15; 16 x 4001 rows in 8 bits 48 of 39 us.  Four CTAs per SM cost it 3 spilled
+// registers at most and gain a resident CTA: three 27.2 and 50.0 us, five (more
+// spills) 27.3 and 50.6.  Reading alone comes to 0.92 of the measured copy rate (32 x
+// 8001 tokens, 65 us).
 template <int BITS, int QUADS>
-__global__ void __launch_bounds__(256) append_kernel(AppendParams p) {
+__global__ void __launch_bounds__(256, QUADS == 4 ? 4 : 1) append_kernel(AppendParams p) {
   pdl_prologue();
   using B = Block<BITS>;
   const int lane = threadIdx.x & 31, w = lane & 7;
