@@ -4,6 +4,7 @@ import ctypes
 
 import numpy as np
 import pytest
+import torch
 
 from oracle import kvcache_ref as R
 from vla_b200 import _lib
@@ -115,3 +116,16 @@ def test_held_values_are_bf16_and_near(bits, most):
     off = np.abs(held - x) / step
     clipped = (codes == 7) & (bits == 4)  # the sign without a code 8 may lose up to a whole step
     assert off[~clipped].max() <= most and off.max() <= 1.0
+
+
+def test_tables_with_overlapping_rows_are_refused():
+    """The kernels take row b at b * stride: one row for all sequences has no such stride."""
+    from vla_b200.kvcache import KVCache, block_bytes
+    pool = torch.zeros(4, 1, block_bytes(4), dtype=torch.uint8)
+    row = torch.arange(3, dtype=torch.int32)
+    for table in (row.expand(5, 3), torch.arange(8, dtype=torch.int32).as_strided((3, 4), (2, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            KVCache.wrap(pool, table, 1, 4)
+    for table in (row.expand(1, 3), torch.zeros(2, 4, dtype=torch.int32)[:, :3], row.expand(5, 3).contiguous()):
+        with pytest.raises(ValueError, match="CUDA"):  # nothing but the device is wrong
+            KVCache.wrap(pool, table, 1, 4)

@@ -77,6 +77,9 @@ class KVCache:
                              f"{pool.dtype} {tuple(pool.shape)}")
         if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError("table: need int32 [batch, max_pages] with unit column stride")
+        if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+            raise ValueError(f"table: rows of {table.shape[1]} page numbers overlap at stride {table.stride(0)}: "
+                             "need a table with rows of its own, .contiguous()")
         if table.device != pool.device or not pool.is_cuda:
             raise ValueError(f"table is on {table.device}, the pool on {pool.device}: need one CUDA device")
         self.pool, self.table = pool, table
@@ -89,7 +92,7 @@ class KVCache:
         for i in range(self.layers):
             d = _lib.KVCacheDesc()
             d.pool, d.table = pool[i].data_ptr(), table.data_ptr()
-            d.table_ld = max(table.stride(0), self.max_pages)
+            d.table_ld = max(table.stride(0), self.max_pages)  # a single row may have any stride
             d.pages, d.max_pages, d.batch = pool.shape[1], self.max_pages, self.batch
             d.kv_heads, d.head_dim, d.bits = kv_heads, HEAD_DIM, bits
             self._desc.append((d, ctypes.byref(d)))
