@@ -499,3 +499,27 @@ def test_many_rows_short_caches_with_empty_sequences(cuda, lens, q_len, room, bi
     share's start, middle and end; rows that do not fill a block."""
     run_case((17, 6, 3, lens, q_len, True, 0, 0), bits, room=room)
     run_case((17, 6, 2, lens, q_len, False, 70, 3), bits, room=room)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("rows,heads", [(1, 3), (5, 12), (90, 3)])
+@pytest.mark.parametrize("raw", [0x7F00, 0x7F7F, 0xFF7F, 0x7E00])
+def test_hidden_slots_that_no_append_wrote(cuda, rows, heads, bits, raw):
+    """Only the first tokens and the newest part of a stream were moved into the cache: the slots below the
+    length that nothing wrote, and that the masks hide, may hold finite scales whose values overflow."""
+    n, window, sinks = 330, 20, 9
+    first = n - rows - window  # the oldest key that the window shows, and one to spare
+    outs = []
+    for fill in (raw, 0):
+        cache, gen = make(1, n, 1, bits, seed=4)
+        cache.pool[..., -512:].view(torch.int16).fill_(fill - 65536 if fill > 32767 else fill)
+        k, v = rows_like(gen, 1, n, 64), rows_like(gen, 1, n, 64)
+        q = rows_like(gen, 1, rows, heads, 64)
+        cache.append(k[:, :sinks].cuda(), v[:, :sinks].cuda(), i32([0]), sinks)
+        cache.append(k[:, first:].cuda(), v[:, first:].cuda(), i32([first]), n - first)
+        outs.append(cache.attend(q.cuda(), i32([n]), window=window, sinks=sinks))
+    hk, hv = (R.held(f64(x).reshape(1, n, 1, 64), bits) for x in (k, v))
+    want, mag, big = R.attend(f64(q), hk, hv, [n], True, window, sinks)
+    assert np.all(np.abs(f64(outs[0]) - want) <= R.attend_bound(want, mag, big))
+    assert torch.equal(outs[0], outs[1])
+    check_clean()

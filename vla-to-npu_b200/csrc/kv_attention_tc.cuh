@@ -45,7 +45,9 @@
 // its value has the probability 0, and 0 times a value must be 0: slots past a
 // sequence's length are written as zeros, and a value group whose scale is NaN
 // (an input's NaN or infinity) is written as zeros and flagged, and the rows
-// that see it are made NaN at the end.
+// that see it are made NaN at the end.  A slot that no append wrote may hold a
+// finite scale whose products leave bf16 (append writes none): they are held to
+// its largest number.
 #pragma once
 #include "attention_tc.cuh"
 #include "kv_attention.cuh"
@@ -78,6 +80,11 @@ struct Raw {
   static constexpr int kBytes = 2 * kCodes + 128;
   static constexpr int kStages = 3;
 };
+
+// Exponent field of a scale from which on a code (at most 8, or 128) times the
+// scale may be 2^128 or more; NaN and the infinities (255) are above it.
+template <int BITS>
+constexpr uint32_t kBigScale = BITS == 4 ? 252u : 248u;
 
 struct Flags {              // per page of a unit
   uint16_t nan[2][2][4];    // [page][value group][tile]: keys whose scale is NaN
@@ -133,6 +140,10 @@ __device__ __forceinline__ void sts8(uint32_t a, uint32_t x, uint32_t y) {
   asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ uint32_t times(uint32_t x, uint32_t d2) { return as_u32(__hmul2(as_bf2(x), as_bf2(d2))); }
+// x held to bf16's finite numbers (not for NaN)
+__device__ __forceinline__ uint32_t finite(uint32_t x) {
+  return as_u32(__hmax2(__hmin2(as_bf2(x), as_bf2(0x7F7F7F7Fu)), as_bf2(0xFF7FFF7Fu)));
+}
 // both halves: the low (high) half of x
 __device__ __forceinline__ uint32_t lo2(uint32_t x) { return __byte_perm(x, x, 0x1010); }
 __device__ __forceinline__ uint32_t hi2(uint32_t x) { return __byte_perm(x, x, 0x3232); }
@@ -535,9 +546,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("ld.shared.u32 %0, [%1];"
                        : "=r"(s)
                        : "r"(from + 2 * Rw::kCodes + (2 * ((lane & 15) >> 2) + (lane & 1)) * 16 + ((lane >> 1) & 1) * 8 + 4));
-          n0 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F80u) == 0x7F80u);
-          n1 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F800000u) == 0x7F800000u);
+          n0 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F80u) >= kBigScale<BITS> << 7);
+          n1 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F800000u) >= kBigScale<BITS> << 23);
           convert<BITS>(from, kt, vt, w * 16, live, live == 16 && (n0 | n1) == 0u, p.mask, lane);
+          if ((n0 | n1) != 0u) {  // rare: of these the NaN are flagged, the others' products held finite
+            n0 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F80u) == 0x7F80u);
+            n1 = __ballot_sync(0xffffffffu, lane < live && (s & 0x7F800000u) == 0x7F800000u);
+            __syncwarp();  // the warp's rows are written
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t at = vt + w * 2048 + i * 512 + lane * 16;
+              const uint4 x = lds16(at);
+              sts16(at, finite(x.x), finite(x.y), finite(x.z), finite(x.w));
+            }
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
