@@ -1,0 +1,60 @@
+"""The streaming text layers without a GPU: where their calls go, by stand-ins that
+record the device that is current when each is made."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from vla_b200 import streaming
+from vla_b200.configs import TextCfg
+
+BF16 = torch.bfloat16
+
+
+class Devices:
+    """torch.cuda.device in place of the real one: the devices entered, innermost last."""
+
+    def __init__(self):
+        self.entered = ["the caller's"]
+
+    def __call__(self, d):
+        outer = self
+
+        class Guard:
+            def __enter__(self):
+                outer.entered.append(d)
+
+            def __exit__(self, *_):
+                outer.entered.pop()
+        return Guard()
+
+
+@pytest.fixture
+def stream(monkeypatch):
+    """A StreamingText of two layers on stand-ins, and the list of its calls with their device."""
+    devices, calls = Devices(), []
+    note = lambda name: lambda *a, **k: calls.append((name, devices.entered[-1]))  # noqa: E731
+    cache = SimpleNamespace(append=note("append"), attend=note("attend"), read=note("read"))
+    layer = SimpleNamespace(**{w: None for w in ("norm1", "norm2", "w_qkv", "w_o", "w_gu", "w_down")})
+    monkeypatch.setattr(torch.cuda, "device", devices)
+    monkeypatch.setattr(streaming, "KVCache", lambda *a, **k: cache)
+    monkeypatch.setattr(streaming, "LlamaLayerWeights", lambda *a, **k: layer)
+    monkeypatch.setattr(streaming, "dev", SimpleNamespace(
+        rms_norm=note("rms_norm"), gemm=note("gemm"), make_epilogue=lambda **k: None))
+    cfg = TextCfg(hidden=192, heads=6, kv_heads=2, head_dim=64, ffn=320, layers=2)
+    return streaming.StreamingText(cfg, [{}, {}], 2, 10, device="cpu"), calls, devices
+
+
+def test_every_launch_of_a_step_is_made_under_its_own_device(stream):
+    text, calls, devices = stream
+    text.step(torch.zeros(2 * 3, 192, dtype=BF16))
+    assert [c for c, _ in calls].count("gemm") == 8 and [c for c, _ in calls].count("attend") == 2
+    assert {d for _, d in calls} == {torch.device("cpu")}, "a launch went to the device that was current"
+    assert devices.entered == ["the caller's"] and text.pos == 3 and text.lens.tolist() == [3, 3]
+
+
+def test_rows_of_another_device_are_refused(stream):
+    text, calls, _ = stream
+    with pytest.raises(ValueError, match="meta"):
+        text.step(torch.zeros(2 * 3, 192, dtype=BF16, device="meta"))
+    assert not calls and text.pos == 0

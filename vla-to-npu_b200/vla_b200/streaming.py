@@ -30,7 +30,8 @@ class StreamingText:
     """``layers`` text layers for ``batch`` streams that advance together.
 
     ``window`` = 0 keeps every token visible; otherwise a token sees the last
-    ``window`` ones and the first ``sinks``.  ``max_len`` tokens fit a stream."""
+    ``window`` ones and the first ``sinks``.  ``max_len`` tokens fit a stream.
+    Steps run on ``device``, on its current stream, whichever device is current."""
 
     def __init__(self, cfg: TextCfg, layers: Sequence[Dict[str, torch.Tensor]], batch: int, max_len: int, bits: int = 4,
                  window: int = 0, sinks: int = 0, device="cuda"):
@@ -60,14 +61,22 @@ class StreamingText:
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """The next n tokens of every stream: x bfloat16 [batch * n, hidden] in
         place through all layers."""
-        c, B = self.cfg, self.batch
-        if x.dim() != 2 or x.shape[1] != c.hidden or x.shape[0] % B or x.dtype != BF16:
-            raise ValueError(f"x: need bfloat16 [{B} * n, {c.hidden}], got {x.dtype} {tuple(x.shape)}")
+        c, B, d = self.cfg, self.batch, self.lens.device
+        if x.dim() != 2 or x.shape[1] != c.hidden or x.shape[0] % B or x.dtype != BF16 or x.device != d:
+            raise ValueError(f"x: need bfloat16 [{B} * n, {c.hidden}] on {d}, got {x.dtype} {tuple(x.shape)} on {x.device}")
         n = x.shape[0] // B
         if self.pos + n > self.max_len:
             raise ValueError(f"{self.pos} + {n} tokens do not fit max_len {self.max_len}")
         if n == 0:
             return x
+        with torch.cuda.device(d):  # the products and norms launch on the current device
+            lens = self._advance(x, n)
+        self.lens = lens
+        self.pos += n
+        return x
+
+    def _advance(self, x: torch.Tensor, n: int) -> torch.Tensor:
+        c, B = self.cfg, self.batch
         self._allocate(B * n)
         lens = self.lens + n
         q = self.qkv.view(B, n, -1)[:, :, :c.q_dim]
@@ -85,9 +94,7 @@ class StreamingText:
             dev.rms_norm(x, lw.norm2, c.eps, out=self.h)
             dev.gemm(self.h, lw.w_gu, self.gu, dev.make_epilogue(act=_lib.ACT_SWIGLU, b_static=True))
             dev.gemm(self.gu, lw.w_down, x, add)
-        self.lens = lens
-        self.pos += n
-        return x
+        return lens
 
     def held(self, layer: int, first: int = 0, n: Optional[int] = None):
         """The keys and values that a layer's cache stands for, bfloat16
