@@ -89,7 +89,8 @@ typedef struct vla_epilogue {
 const char* vla_last_error(void);
 int vla_version(void);
 /* Synchronises the current device, then reads and clears the device error
- * word.  Returns VLA_OK, VLA_E_DEVICE_TIMEOUT, VLA_E_DEVICE_RANGE or VLA_E_CUDA. */
+ * word.  Returns VLA_OK, VLA_E_DEVICE_TIMEOUT, VLA_E_DEVICE_RANGE (only where no
+ * wait expired) or VLA_E_CUDA. */
 int vla_sync_check(void);
 /* Device error word without clearing (0 = none). */
 int vla_peek_device_error(unsigned int* code);

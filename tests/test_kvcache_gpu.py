@@ -523,3 +523,34 @@ def test_hidden_slots_that_no_append_wrote(cuda, rows, heads, bits, raw):
     assert np.all(np.abs(f64(outs[0]) - want) <= R.attend_bound(want, mag, big))
     assert torch.equal(outs[0], outs[1])
     check_clean()
+
+
+def test_an_expired_wait_outranks_a_skipped_page(cuda):
+    """A page that was skipped must not hide that a kernel gave up, whichever came first."""
+    import ctypes
+    from vla_b200 import _lib
+    from vla_b200.kvcache import KVCache
+    lib = _lib.load()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    cache = KVCache(1, 64, kv_heads=1, pages=1)  # its table holds no page
+    q = torch.zeros(1, 1, 3, 64, dtype=BF16, device="cuda")
+    check_clean()
+    for order in ("page wait", "wait page"):
+        for what in order.split():
+            if what == "page":
+                cache.attend(q, i32([5]))
+            else:
+                _lib.check(lib.vla_test_expired_wait(1000, stream))  # 1 ms limit
+            torch.cuda.synchronize()
+        code = ctypes.c_uint(0)
+        _lib.check(lib.vla_peek_device_error(ctypes.byref(code)))
+        assert code.value == 0x1FF
+        assert lib.vla_sync_check() == _lib.VLA_E_DEVICE_TIMEOUT
+        assert "0x1ff" in _lib.last_error()
+        check_clean()
+    cache.attend(q, i32([5]))
+    torch.cuda.synchronize()
+    _lib.check(lib.vla_peek_device_error(ctypes.byref(code)))
+    assert code.value == 0x301
+    assert lib.vla_sync_check() == _lib.VLA_E_DEVICE_RANGE
+    check_clean()

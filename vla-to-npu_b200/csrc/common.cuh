@@ -16,6 +16,9 @@ typedef __nv_bfloat16 bf16;
 // clears it with vla_sync_check().
 // --------------------------------------------------------------------------
 __device__ unsigned int g_vla_device_error = 0;
+// Set where a kernel skipped a cache position or page: a word of its own, so that
+// it never stands in the way of an expired wait, which leaves outputs unwritten.
+__device__ unsigned int g_vla_device_range = 0;
 
 enum : unsigned int {
   VLA_DERR_NONE = 0,
@@ -41,6 +44,7 @@ __device__ __forceinline__ uint64_t vla_globaltimer() {
 __device__ __forceinline__ void vla_record_error(unsigned int code) {
   atomicCAS(&g_vla_device_error, 0u, code);
 }
+__device__ __forceinline__ void vla_record_range() { atomicExch(&g_vla_device_range, (unsigned int)VLA_DERR_KV_RANGE); }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -73,7 +73,7 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int r0, int 
   s.len = p.lens[b];
   const long long room = (long long)p.c.max_pages * kPage;
   if (s.len < 0 || s.len > room) {
-    vla_record_error(VLA_DERR_KV_RANGE);
+    vla_record_range();
     s.len = s.len < 0 ? 0 : (int)room;
   }
   s.ql = p.q_len != nullptr ? max(0, min(p.Lq, p.q_len[b])) : p.Lq;
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
   auto block = [&](int u, int page) -> const uint8_t* {
     if (u >= u1) return nullptr;
     if (page < 0 || page >= p.c.pages) {
-      vla_record_error(VLA_DERR_KV_RANGE);
+      vla_record_range();
       return nullptr;
     }
     return p.c.pool + ((long long)page * heads + h) * Block<BITS>::kBytes;

@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (lane < 8)
                 copy16(dst + 2 * Rw::kCodes, blk + Block<BITS>::kScales + (w & 3) * 128 + lane * 16);
             } else {
-              vla_record_error(VLA_DERR_KV_RANGE);
+              vla_record_range();
             }
           }
           there = have ? there | (1u << st) : there & ~(1u << st);

@@ -66,12 +66,12 @@ struct Cache {
 template <int BITS>
 __device__ __forceinline__ uint8_t* block_of(const Cache& c, int b, int slot, int h) {
   if (slot < 0 || slot >= c.max_pages) {
-    vla_record_error(VLA_DERR_KV_RANGE);
+    vla_record_range();
     return nullptr;
   }
   const int page = c.table[(long long)b * c.table_ld + slot];
   if (page < 0 || page >= c.pages) {
-    vla_record_error(VLA_DERR_KV_RANGE);
+    vla_record_range();
     return nullptr;
   }
   return c.pool + ((long long)page * c.kv_heads + h) * Block<BITS>::kBytes;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(256, QUADS == 4 ? 4 : 1) append_kernel(AppendP
   for (int b = blockIdx.y; b < p.c.batch; b += gridDim.y) {
     const int s = p.start[b];
     const int valid = p.count != nullptr ? min(p.n, p.count[b]) : p.n;
-    if (s < 0) vla_record_error(VLA_DERR_KV_RANGE);
+    if (s < 0) vla_record_range();
     const bf16* kb = p.k + (long long)b * p.k_batch + h * HD + w * 8;
     const bf16* vb = p.v + (long long)b * p.v_batch + h * HD + w * 8;
     Lane it[QUADS];
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(256) read_kernel(ReadParams p) {
   for (int b = blockIdx.y; b < p.c.batch; b += gridDim.y) {
     const int s = p.start != nullptr ? p.start[b] : 0;
     const int valid = p.count != nullptr ? min(p.n, p.count[b]) : p.n;
-    if (s < 0) vla_record_error(VLA_DERR_KV_RANGE);
+    if (s < 0) vla_record_range();
     bf16* kd = p.k + (long long)b * p.k_batch + h * HD + w * 8;
     bf16* vd = p.v + (long long)b * p.v_batch + h * HD + w * 8;
     Lane it[QUADS];

@@ -87,20 +87,23 @@ int vla_version(void) { return 100; }
 
 int vla_sync_check(void) {
   VLA_CUDA_TRY(cudaDeviceSynchronize());
-  unsigned int code = 0, zero = 0;
+  unsigned int code = 0, range = 0, zero = 0;
   VLA_CUDA_TRY(cudaMemcpyFromSymbol(&code, g_vla_device_error, sizeof(code)));
-  if (code != 0) {
-    VLA_CUDA_TRY(cudaMemcpyToSymbol(g_vla_device_error, &zero, sizeof(zero)));
-    if (code == VLA_DERR_KV_RANGE)
-      return set_error(VLA_E_DEVICE_RANGE, "a cache position, length or page number was out of range (code 0x%x)", code);
-    return set_error(VLA_E_DEVICE_TIMEOUT, "device wait limit expired (code 0x%x)", code);
-  }
+  VLA_CUDA_TRY(cudaMemcpyFromSymbol(&range, g_vla_device_range, sizeof(range)));
+  if (code != 0) VLA_CUDA_TRY(cudaMemcpyToSymbol(g_vla_device_error, &zero, sizeof(zero)));
+  if (range != 0) VLA_CUDA_TRY(cudaMemcpyToSymbol(g_vla_device_range, &zero, sizeof(zero)));
+  if (code != 0)
+    return set_error(VLA_E_DEVICE_TIMEOUT, "device wait limit expired (code 0x%x)%s", code,
+                     range != 0 ? "; a cache position, length or page number was out of range, too" : "");
+  if (range != 0)
+    return set_error(VLA_E_DEVICE_RANGE, "a cache position, length or page number was out of range (code 0x%x)", range);
   return VLA_OK;
 }
 
 int vla_peek_device_error(unsigned int* code) {
   VLA_CHECK_ARG(code != nullptr, "null code");
   VLA_CUDA_TRY(cudaMemcpyFromSymbol(code, g_vla_device_error, sizeof(*code)));
+  if (*code == 0) VLA_CUDA_TRY(cudaMemcpyFromSymbol(code, g_vla_device_range, sizeof(*code)));
   return VLA_OK;
 }
 
