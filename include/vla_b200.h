@@ -340,7 +340,7 @@ int vla_kv_append_bf16(const vla_kv_cache* c, const void* k, int64_t k_row, int6
 
 /* The bf16 keys and values that the cache stands for: token start[b] + i (start
  * NULL: 0) to row i < n of sequence b; rows i >= count[b] (NULL: n) are written
- * as zeros. */
+ * as zeros.  The strides must keep all rows apart. */
 int vla_kv_read_bf16(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, void* v, int64_t v_row,
                      int64_t v_batch, int32_t n, const int32_t* start, const int32_t* count, vla_stream_t stream);
 
@@ -351,7 +351,8 @@ int vla_kv_read_bf16(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_ba
  * causal, else every one has lens[b] - 1.  A query at position p sees key j <= p
  * when window == 0 or j > p - window or j < sinks.  Rows that see no key, and
  * rows i >= q_len[b], are written as zeros.  Keys that are not seen have no
- * effect, whatever their memory holds.
+ * effect, whatever their memory holds.  Sequences may share queries (q_batch 0);
+ * their outputs must lie apart.
  * max_len (0: the table's capacity) is an upper bound of lens that the split of
  * the work is made for; longer sequences stay right.  The workspace
  * (vla_kv_attention_workspace bytes, 16-byte aligned; 0: none) holds the parts'

@@ -129,3 +129,26 @@ def test_tables_with_overlapping_rows_are_refused():
     for table in (row.expand(1, 3), torch.zeros(2, 4, dtype=torch.int32)[:, :3], row.expand(5, 3).contiguous()):
         with pytest.raises(ValueError, match="CUDA"):  # nothing but the device is wrong
             KVCache.wrap(pool, table, 1, 4)
+
+
+@pytest.mark.parametrize("n,row,batch", [
+    (1, 320, 0), (4, 320, 0),          # one sequence's rows for all
+    (1, 320, 312), (4, 320, 1272),     # the last 8 elements are shared
+    (4, 640, 312), (4, 632, 320),      # rows of all sequences in turn, too close
+])
+def test_outputs_that_overlap_are_refused(n, row, batch):
+    """Two sequences with a row in common would be written by two writers."""
+    lib, d = _lib.load(), ctypes.byref(cache_desc())
+    assert lib.vla_kv_read_bf16(d, 256, row, batch, 4096, 320, 1280, n, None, None, None) == _lib.VLA_E_INVALID
+    assert "k overlap" in _lib.last_error()
+    assert lib.vla_kv_read_bf16(d, 256, 320, 1280, 4096, row, batch, n, None, None, None) == _lib.VLA_E_INVALID
+    assert "v overlap" in _lib.last_error()
+    a = attention_args(Lq=n, Hq=5, q_row=320, q_batch=0, o_row=row, o_batch=batch)
+    assert lib.vla_kv_attention_bf16(d, ctypes.byref(a), None) == _lib.VLA_E_INVALID
+    assert "o overlap" in _lib.last_error()
+
+
+def test_one_output_for_keys_and_values_is_refused():
+    lib, d = _lib.load(), ctypes.byref(cache_desc())
+    assert lib.vla_kv_read_bf16(d, 256, 320, 1280, 256, 320, 1280, 4, None, None, None) == _lib.VLA_E_INVALID
+    assert "one output" in _lib.last_error()

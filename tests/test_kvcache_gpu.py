@@ -554,3 +554,25 @@ def test_an_expired_wait_outranks_a_skipped_page(cuda):
     assert code.value == 0x301
     assert lib.vla_sync_check() == _lib.VLA_E_DEVICE_RANGE
     check_clean()
+
+
+def test_outputs_may_lie_between_each_other(cuda):
+    """Keys and values in one buffer, and the rows of all sequences in turn (token-major): no element has two writers."""
+    from vla_b200 import _lib
+    B, n, H = 3, 20, 2
+    cache, gen = make(B, n, H, 4)
+    k, v = rows_like(gen, B, n, H * 64), rows_like(gen, B, n, H * 64)
+    cache.append(k.cuda(), v.cuda(), i32([0] * B), n)
+    buf = torch.zeros(n, B, 2, H * 64, dtype=BF16, device="cuda")
+    views = buf[:, :, 0].transpose(0, 1), buf[:, :, 1].transpose(0, 1)
+    for got, want in zip(cache.read(n, out=views), cache.read(n)):
+        assert torch.equal(got, want)
+    q, lens = rows_like(gen, B, n, 6, 64).cuda(), i32([n] * B)
+    out = torch.zeros(n, B, 6 * 64, dtype=BF16, device="cuda").transpose(0, 1)
+    assert torch.equal(cache.attend(q, lens, out=out), cache.attend(q, lens).flatten(2))
+    one = torch.zeros(1, n, 6 * 64, dtype=BF16, device="cuda").expand(B, n, 6 * 64)
+    with pytest.raises(_lib.VlaError, match="overlap"):
+        cache.attend(q, lens, out=one)
+    with pytest.raises(_lib.VlaError, match="overlap"):
+        cache.read(n, out=(one[..., :128], torch.zeros(B, n, 128, dtype=BF16, device="cuda")))
+    check_clean()

@@ -43,6 +43,18 @@ static int check_rows(const void* x, int64_t row, int64_t batch, int64_t width, 
   return VLA_OK;
 }
 
+// Output rows: no element may have two writers.  Sequences lie one after the
+// other, or (rows of all sequences, then the next row of all) within a row's stride.
+static int check_apart(const vla_kv_cache* c, int64_t n, int64_t row, int64_t batch, int64_t width, const char* what,
+                       const char* name) {
+  const int64_t b = c->batch - 1;
+  VLA_CHECK_ARG(b == 0 || (batch >= width && (batch - width) / row >= n - 1) ||
+                    (batch >= width && (row - width) / batch >= b),
+                "%s: sequences of %s overlap: %lld rows of %lld elements, strides %lld and %lld", what, name,
+                (long long)n, (long long)width, (long long)row, (long long)batch);
+  return VLA_OK;
+}
+
 // Whether four groups of positions per warp leave a warp for each of the SMs' 64 places.
 static bool wide_rows(const vla_kv_cache* c, int quads) {
   return (long long)c->batch * c->kv_heads * ((quads + 3ll) / 4) >= 64ll * device_info().num_sms;
@@ -86,6 +98,9 @@ static int read(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_batch, 
   const int64_t width = (int64_t)c->kv_heads * HD;
   VLA_TRY(check_rows(k, k_row, k_batch, width, "kv_read", "k"));
   VLA_TRY(check_rows(v, v_row, v_batch, width, "kv_read", "v"));
+  VLA_TRY(check_apart(c, n, k_row, k_batch, width, "kv_read", "k"));
+  VLA_TRY(check_apart(c, n, v_row, v_batch, width, "kv_read", "v"));
+  VLA_CHECK_ARG(k != v, "kv_read: k and v are one output");
   ReadParams p{device_cache(c), (bf16*)k, (bf16*)v, (long long)k_row, (long long)v_row, (long long)k_batch,
                (long long)v_batch, start, count, n, (int)(((long long)n + 6) / 4),
                c->bits == 4 ? code_mask<4>() : code_mask<8>()};
@@ -220,6 +235,7 @@ static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cuda
   VLA_CHECK_ARG(a->lens != nullptr, "kv_attention: null lens");
   VLA_TRY(check_rows(a->q, a->q_row, a->q_batch, (int64_t)a->Hq * HD, "kv_attention", "q"));
   VLA_TRY(check_rows(a->o, a->o_row, a->o_batch, (int64_t)a->Hq * HD, "kv_attention", "o"));
+  VLA_TRY(check_apart(c, a->Lq, a->o_row, a->o_batch, (int64_t)a->Hq * HD, "kv_attention", "o"));
   Plan pl;
   VLA_TRY(plan_attention(c, a, &pl));
   if (pl.workspace > 0) {
