@@ -576,3 +576,18 @@ def test_outputs_may_lie_between_each_other(cuda):
     with pytest.raises(_lib.VlaError, match="overlap"):
         cache.read(n, out=(one[..., :128], torch.zeros(B, n, 128, dtype=BF16, device="cuda")))
     check_clean()
+
+
+def test_a_refused_call_leaves_the_next_one_alone(cuda):
+    """A call whose arguments are refused says nothing about the workspace of valid ones of its sizes."""
+    from vla_b200 import _lib
+    cache, gen = make(1, 3000, 1, 4)
+    k, v = rows_like(gen, 1, 3000, 64), rows_like(gen, 1, 3000, 64)
+    cache.append(k.cuda(), v.cuda(), i32([0]), 3000)
+    for rows in (1, 40):  # either kernel, both split along the cache
+        q, lens = rows_like(gen, 1, rows, 3, 64).cuda(), i32([3000])
+        for scale in (float("nan"), 0.0):
+            with pytest.raises(_lib.VlaError, match="scale"):
+                cache.attend(q, lens, scale=scale)
+        got = cache.attend(q, lens)
+        assert torch.equal(got, cache.attend(q, lens, max_len=3001))  # a plan of its own

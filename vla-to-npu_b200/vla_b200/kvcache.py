@@ -204,13 +204,16 @@ class KVCache:
         desc, args = self._desc[layer][1], ctypes.byref(a)
         key = (n, heads, window, sinks, max_len)
         need = self._plans.get(key)
-        if need is None:
-            if len(self._plans) >= 4096:
-                self._plans.clear()
+        new = need is None
+        if new:
             with torch.cuda.device(self._dev):
-                need = self._plans[key] = self._lib.vla_kv_attention_workspace(desc, args)
+                need = self._lib.vla_kv_attention_workspace(desc, args)
         if need:
             ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=self.device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         self._call(self._attend, desc, args)
+        if new:  # (0 bytes is also the answer to a call that is refused)
+            if len(self._plans) >= 4096:
+                self._plans.clear()
+            self._plans[key] = need
         return out
