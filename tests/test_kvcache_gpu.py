@@ -591,3 +591,34 @@ def test_a_refused_call_leaves_the_next_one_alone(cuda):
                 cache.attend(q, lens, scale=scale)
         got = cache.attend(q, lens)
         assert torch.equal(got, cache.attend(q, lens, max_len=3001))  # a plan of its own
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_special_values_are_written_as_defined(cuda, bits):
+    """The bytes of groups where a rounding or a sign can go wrong: the scales, and the
+    codes wherever the scale is a number."""
+    from vla_b200.kvcache import KVCache
+    x = special_rows()
+    y = x.roll(32, dims=1)
+    n = len(x)
+    cache = KVCache(1, n, kv_heads=1, bits=bits)
+    cache.append(x.cuda(), y.cuda(), i32([0]), n)
+    got = cache.pool[0, :, 0].cpu().numpy()
+    want = got.copy()
+    for i in range(n):
+        R.write_token(want[i // 64], bits, i % 64, f64(x)[i], f64(y)[i])
+    for i in range(n):
+        for keys, rows in ((True, x), (False, y)):
+            for group in range(2):
+                at = R.scale_place(bits, keys, i % 64, group)
+                np.testing.assert_array_equal(got[i // 64, at:at + 2], want[i // 64, at:at + 2], f"{rows[i]}")
+                if got[i // 64, at + 1] == 0x7F and got[i // 64, at] & 0x80:
+                    continue  # NaN
+                places = {R.code_place(bits, keys, i % 64, 32 * group + d) for d in range(32)}
+                for byte, shift in places:
+                    m = 15 << shift if bits == 4 else 255
+                    assert got[i // 64, byte] & m == want[i // 64, byte] & m, (rows[i], byte, shift)
+    for back, rows in zip(cache.read(n), (x, y)):  # zeros with their signs
+        held = R.held(f64(rows), bits)
+        same = np.signbit(f64(back[0])) == np.signbit(held)
+        assert np.all(same | np.isnan(held))

@@ -117,7 +117,7 @@ __device__ __forceinline__ void codes8(uint32_t w, uint32_t mask, uint32_t* p) {
 }
 
 // Scale of a group from its largest positive and largest negative magnitude
-// (bf16 bits, the larger one >= 0).
+// (bf16 bits; below 0 where no element has that sign, but the larger one >= 0).
 template <int BITS>
 __device__ __forceinline__ float group_scale(int hp, int hn) {
   const int top = max(hp, hn);
@@ -127,7 +127,7 @@ __device__ __forceinline__ float group_scale(int hp, int hn) {
     // a / 8 up to 5 significant bits: 4 of the 23 mantissa bits stay
     d = __uint_as_float((__float_as_uint(a * 0.125f) + 0x0007FFFFu) & ~0x0007FFFFu);
     d = fmaxf(d, 0x1p-100f);
-    if (hp > hn) d = -d;
+    if (hp > max(hn, 0)) d = -d;
   } else {
     // a in [2^k, 2^(k+1)): 127 * 2^(k-6) reaches it or 127 * 2^(k-5) does
     const float p = __uint_as_float(__float_as_uint(a) & 0x7F800000u) * 0x1p-6f;
