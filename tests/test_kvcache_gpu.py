@@ -622,3 +622,17 @@ def test_special_values_are_written_as_defined(cuda, bits):
         held = R.held(f64(rows), bits)
         same = np.signbit(f64(back[0])) == np.signbit(held)
         assert np.all(same | np.isnan(held))
+
+
+@pytest.mark.parametrize("scale", [1e-36, 1e-38, 1e-42])
+@pytest.mark.parametrize("rows,n", [(1, 300), (1, 3000), (7, 700), (40, 300)])
+def test_scales_near_zero_give_the_mean(cuda, rows, n, scale):
+    """Every positive finite scale counts, also one whose reciprocal is not finite."""
+    cache, gen = make(1, n, 1, 4)
+    k, v = rows_like(gen, 1, n, 64), rows_like(gen, 1, n, 64)
+    cache.append(k.cuda(), v.cuda(), i32([0]), n)
+    q = rows_like(gen, 1, rows, 3, 64)
+    hk, hv = (R.held(f64(x).reshape(1, n, 1, 64), 4) for x in (k, v))
+    want, mag, big = R.attend(f64(q), hk, hv, [n], scale=scale)
+    got = cache.attend(q.cuda(), i32([n]), scale=scale)
+    assert np.all(np.abs(f64(got) - want) <= R.attend_bound(want, mag, big))

@@ -442,7 +442,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(AttnParams p) {
     m[j][0] = m[j][1] = -INFINITY;
     l[j] = ms[j] = make_float2(0.f, 0.f);
   }
-  const float grow = 8.f / p.scale_log2;  // the maximum moves in steps above 2^8 only
+  // the maximum moves in steps above 2^8 only (of raw products; finite also for a scale near 0)
+  const float grow = fminf(8.f / p.scale_log2, 0x1.fffffep127f);
   const uint32_t mask = p.mask;
   const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
 
