@@ -152,3 +152,10 @@ def test_one_output_for_keys_and_values_is_refused():
     lib, d = _lib.load(), ctypes.byref(cache_desc())
     assert lib.vla_kv_read_bf16(d, 256, 320, 1280, 256, 320, 1280, 4, None, None, None) == _lib.VLA_E_INVALID
     assert "one output" in _lib.last_error()
+
+
+def test_a_scale_that_overflows_in_base_two_is_refused():
+    """Exponentials are taken to base 2: the scale times log2(e) has to be a number, too."""
+    a = attention_args(scale=3e38)
+    assert _lib.load().vla_kv_attention_bf16(ctypes.byref(cache_desc()), ctypes.byref(a), None) == _lib.VLA_E_INVALID
+    assert "scale" in _lib.last_error()

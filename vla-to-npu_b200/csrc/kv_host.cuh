@@ -11,6 +11,8 @@
 namespace vla {
 namespace kv {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 static size_t block_bytes(int bits) {
   return bits == 4 ? (size_t)Block<4>::kBytes : bits == 8 ? (size_t)Block<8>::kBytes : 0;
 }
@@ -181,7 +183,8 @@ static int check_attention(const vla_kv_cache* c, const vla_kv_attention_args* a
   VLA_CHECK_ARG(a->Lq >= 0 && a->Hq > 0 && a->Hq % c->kv_heads == 0, "kv_attention: %d query heads over %d kv heads",
                 a->Hq, c->kv_heads);
   VLA_CHECK_ARG(a->window >= 0 && a->sinks >= 0 && a->max_len >= 0, "kv_attention: negative window, sinks or max_len");
-  VLA_CHECK_ARG(std::isfinite(a->scale) && a->scale > 0.f, "kv_attention: scale must be positive and finite");
+  VLA_CHECK_ARG(std::isfinite(a->scale * kLog2e) && a->scale > 0.f,
+                "kv_attention: scale (times log2 e) must be positive and finite");
   return VLA_OK;
 }
 
@@ -261,7 +264,7 @@ static int attention(const vla_kv_cache* c, const vla_kv_attention_args* a, cuda
   const long long room = (long long)c->max_pages * kPage;
   p.window = a->window > 0 && a->window < room ? a->window : 0;
   p.sinks = a->sinks < room ? a->sinks : (int)room;
-  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.scale_log2 = a->scale * kLog2e;
   p.mask = c->bits == 4 ? code_mask<4>() : code_mask<8>();
   p.block = pl.block;
   p.row_blocks = pl.row_blocks;
