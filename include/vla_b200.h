@@ -322,7 +322,7 @@ typedef struct vla_kv_cache {
   const int32_t* table;   /* device [batch][table_ld] */
   int64_t table_ld;
   int32_t pages;          /* pages in the pool */
-  int32_t max_pages;      /* table columns: a sequence holds at most 64 * max_pages tokens */
+  int32_t max_pages;      /* table columns: a sequence holds at most 64 * max_pages tokens, 2^31 - 512 or less */
   int32_t batch, kv_heads;
   int32_t head_dim;       /* 64 */
   int32_t bits;           /* 4 or 8 */

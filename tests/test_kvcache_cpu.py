@@ -159,3 +159,14 @@ def test_a_scale_that_overflows_in_base_two_is_refused():
     a = attention_args(scale=3e38)
     assert _lib.load().vla_kv_attention_bf16(ctypes.byref(cache_desc()), ctypes.byref(a), None) == _lib.VLA_E_INVALID
     assert "scale" in _lib.last_error()
+
+
+def test_tables_whose_windows_could_wrap_are_refused():
+    """A row 255 positions before the first key, less a window of the whole table, has to fit 32 bits."""
+    d = cache_desc(max_pages=(1 << 25) - 7, table_ld=1 << 25)
+    assert _lib.load().vla_kv_attention_bf16(ctypes.byref(d), ctypes.byref(attention_args()), None) == _lib.VLA_E_INVALID
+    assert "2^31 - 512" in _lib.last_error()
+    d.max_pages -= 1
+    a = attention_args()
+    assert _lib.load().vla_kv_attention_workspace(ctypes.byref(d), ctypes.byref(a)) > 0
+    assert -255 - (64 * d.max_pages - 1) + 1 >= -(1 << 31)

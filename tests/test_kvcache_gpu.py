@@ -636,3 +636,22 @@ def test_scales_near_zero_give_the_mean(cuda, rows, n, scale):
     want, mag, big = R.attend(f64(q), hk, hv, [n], scale=scale)
     got = cache.attend(q.cuda(), i32([n]), scale=scale)
     assert np.all(np.abs(f64(got) - want) <= R.attend_bound(want, mag, big))
+
+
+def test_the_longest_window_with_rows_before_the_first_key(cuda):
+    """Queries at negative positions see nothing; their window reaches almost to -2^31."""
+    from vla_b200.kvcache import KVCache
+    gen = torch.Generator().manual_seed(6)
+    room, n = 2 ** 31 - 512, 90
+    cache = KVCache(2, room, kv_heads=1, pages=4)
+    cache.table[:, :2] = torch.tensor([[3, 0], [1, 2]])
+    k, v = rows_like(gen, 2, n, 64), rows_like(gen, 2, n, 64)
+    lens = [30, 90]
+    cache.append(k.cuda(), v.cuda(), i32([0, 0]), n, count=i32(lens))
+    q = rows_like(gen, 2, 100, 3, 64)
+    hk, hv = (R.held(f64(x).reshape(2, n, 1, 64), 4) for x in (k, v))
+    want, mag, big = R.attend(f64(q), hk, hv, lens)
+    got = f64(cache.attend(q.cuda(), i32(lens), window=room - 1))
+    assert np.all(np.abs(got - want) <= R.attend_bound(want, mag, big))
+    assert np.abs(got[0, 70:]).max() > 0 and (got[0, :70] == 0).all()
+    check_clean()

@@ -22,7 +22,8 @@ static int check_cache(const vla_kv_cache* c, const char* what) {
   VLA_CHECK_ARG(c->bits == 4 || c->bits == 8, "%s: a cache holds 4 or 8 bits, not %d", what, c->bits);
   VLA_CHECK_ARG(c->head_dim == HD, "%s: head_dim must be 64", what);
   VLA_CHECK_ARG(c->batch >= 0 && c->kv_heads > 0 && c->pages >= 0 && c->max_pages >= 0, "%s: bad cache shape", what);
-  VLA_CHECK_ARG((long long)c->max_pages * kPage < (1ll << 31), "%s: %d pages per sequence are 2^31 tokens or more",
+  // a block's first row may lie 255 positions before the first key, and its window starts below that
+  VLA_CHECK_ARG((long long)c->max_pages * kPage <= (1ll << 31) - 512, "%s: %d pages per sequence are over 2^31 - 512 tokens",
                 what, c->max_pages);
   VLA_CHECK_ARG(c->table_ld >= c->max_pages, "%s: table stride %lld below its %d columns", what,
                 (long long)c->table_ld, c->max_pages);
