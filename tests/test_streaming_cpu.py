@@ -58,3 +58,15 @@ def test_rows_of_another_device_are_refused(stream):
     with pytest.raises(ValueError, match="meta"):
         text.step(torch.zeros(2 * 3, 192, dtype=BF16, device="meta"))
     assert not calls and text.pos == 0
+
+
+def test_tokens_that_are_not_held_are_refused(stream):
+    text, calls, _ = stream
+    text.step(torch.zeros(2 * 3, 192, dtype=BF16))
+    for first, n in ((0, 4), (2, 2), (-1, 2), (4, None), (0, -1)):
+        with pytest.raises(ValueError, match="tokens"):
+            text.held(0, first, n)
+    assert "read" not in [c for c, _ in calls]
+    text.held(0, 1)
+    text.held(1, 3, 0)
+    assert [c for c, _ in calls].count("read") == 2

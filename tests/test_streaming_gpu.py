@@ -89,3 +89,14 @@ def test_command_line_example_runs(cuda, capsys):
     streaming.main(["--batch", "2", "--steps", "3", "--layers", "2", "--window", "200", "--sinks", "48"])
     out = capsys.readouterr().out
     assert "2 streams x 339 tokens" in out and "held keys off by 0.0" in out
+
+
+def test_held_refuses_tokens_that_are_not_there(cuda):
+    from vla_b200.streaming import StreamingText
+    cfg, params = small()
+    text = StreamingText(cfg, params, 2, 10)
+    text.step(torch.zeros(2 * 6, cfg.hidden, dtype=BF16, device="cuda"))
+    assert text.held(0)[0].shape == (2, 6, 128) and text.held(0, 6)[0].shape == (2, 0, 128)
+    for first, n in ((0, 7), (5, 2), (-1, 3), (7, None), (0, -1)):
+        with pytest.raises(ValueError, match="tokens"):
+            text.held(0, first, n)

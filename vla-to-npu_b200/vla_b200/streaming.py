@@ -100,6 +100,8 @@ class StreamingText:
         """The keys and values that a layer's cache stands for, bfloat16
         [batch, n, kv_dim] each, tokens first .. first + n (all up to now)."""
         n = self.pos - first if n is None else n
+        if first < 0 or n < 0 or first + n > self.pos:
+            raise ValueError(f"tokens {first} .. {first + n}: {self.pos} are held")
         return self.cache.read(n, start=torch.full_like(self.lens, first), layer=layer)
 
 
