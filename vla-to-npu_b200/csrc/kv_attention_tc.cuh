@@ -813,7 +813,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (hf == 0) sm.top[it & 1][at] = m;
       }
       if (!ok) {  // release the row's other warp
-        if (lane == 0) *abort_flag = 1;
+        if (lane == 0) {
+          if (!*abort_flag) vla_record_error(VLA_DERR_ATTN_TIMEOUT);
+          *abort_flag = 1;
+        }
         __syncwarp();
         asm volatile("bar.arrive %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
       }
