@@ -117,6 +117,7 @@ struct Smem {
   uint64_t v_full[kRing], v_empty[kRing];
   uint64_t s_full[kBuffers], s_empty[kBuffers];  // per buffer
   uint64_t p_full[2], pv_done[2];                // per group
+  uint64_t drained[2];                           // S and P.V issuer, after an expired wait
   float swap[2][2][kRows];       // [turn][half of the keys]: maxima that a row's two threads tell each other
   float sum[2][2][kRows], top[2][kRows];  // [segment's parity]: what a segment's rows are finished with
   uint8_t nan[2][2][kRows];
@@ -269,6 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.q_full[i], 16);
       mbar_init(&sm.p_full[i], 256);
       mbar_init(&sm.pv_done[i], 1);
+      mbar_init(&sm.drained[i], 1);
     }
     for (int i = 0; i < kBuffers; ++i) {
       mbar_init(&sm.s_full[i], 1);
@@ -415,6 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j == 0) ok = mbar_wait_bounded(&sm.q_full[qb], (it >> 1) & 1, abort_flag);
             if (ok) ok = mbar_wait_bounded(&sm.k_full[sk], ((tile >> 1) / kRing) & 1, abort_flag);
             if (ok) ok = mbar_wait_bounded(&sm.s_empty[buf], ((tile / kBuffers) & 1) ^ 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);  // (lanes time their waits by themselves)
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
@@ -443,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int tile = 2 * t + j, g = j & 1, buf = tile % kBuffers, sv = (tile >> 1) % kRing;
             ok = mbar_wait_bounded(&sm.p_full[g], (uint32_t)(tile >> 1) & 1u, abort_flag);
             if (ok) ok = mbar_wait_bounded(&sm.v_full[sv], ((tile >> 1) / kRing) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
@@ -461,6 +465,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           t += n;
         }
+      }
+      if (!ok && (warp == 1 || warp == 2)) {  // products in flight end before the TMEM is freed (bounded)
+        if (elect_one()) tc_commit(&sm.drained[warp - 1]);
+        __syncwarp();
+        mbar_wait_bounded(&sm.drained[warp - 1], 0, nullptr, 2000000ull);
       }
     } else if (warp < kSoft0) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCodeRegs));
@@ -599,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float r;
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(smem_u32(&sm.swap[turn & 1][hf ^ 1][at])));
         ++turn;
-        if (*abort_flag) ok = false;  // (raised before the other warp gave up)
+        ok = !__any_sync(0xffffffffu, *abort_flag);  // (raised before the other warp gave up)
         return r;
       };
       auto queries_there = [&]() {  // of the next segment
@@ -812,7 +821,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm.nan[it & 1][hf][at] = (uint8_t)nan;
         if (hf == 0) sm.top[it & 1][at] = m;
       }
-      if (!ok) {  // release the row's other warp
+      if (!ok) {  // the queries in flight land; release the row's other warp
+        copy_wait<0>();
         if (lane == 0) {
           if (!*abort_flag) vla_record_error(VLA_DERR_ATTN_TIMEOUT);
           *abort_flag = 1;
