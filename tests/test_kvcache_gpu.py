@@ -655,3 +655,61 @@ def test_the_longest_window_with_rows_before_the_first_key(cuda):
     assert np.all(np.abs(got - want) <= R.attend_bound(want, mag, big))
     assert np.abs(got[0, 70:]).max() > 0 and (got[0, :70] == 0).all()
     check_clean()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_append_and_read_of_calls_that_fill_the_gpu(cuda, bits):
+    """Four groups of positions per warp (calls of 64 warps per SM and more): bytes and values, uneven starts and counts."""
+    B, n, H = 320, 113, 5
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert B * H * -(-((n + 6) // 4) // 4) >= 64 * sms
+    starts = [37 * b % 70 for b in range(B)]
+    counts = [n if b % 40 == 3 else b % 7 for b in range(B)]
+    cache, gen = make(B, 70 + n, H, bits, spare=3)
+    want = cache.pool[0].cpu().numpy().copy()
+    k, v = rows_like(gen, B, n, H * 64), rows_like(gen, B, n, H * 64)
+    cache.append(k.cuda(), v.cuda(), i32(starts), n, count=i32(counts))
+    table, kk, vv = cache.table.cpu().numpy(), f64(k).reshape(B, n, H, 64), f64(v).reshape(B, n, H, 64)
+    held = np.zeros((2, B, n, H, 64))
+    for b in range(B):
+        for i in range(counts[b]):
+            at = starts[b] + i
+            for h in range(H):
+                R.write_token(want[table[b, at // 64], h], bits, at % 64, kk[b, i, h], vv[b, i, h])
+        held[0, b, :counts[b]], held[1, b, :counts[b]] = R.held(kk[b, :counts[b]], bits), R.held(vv[b, :counts[b]], bits)
+    np.testing.assert_array_equal(cache.pool[0].cpu().numpy(), want)
+    for got, x in zip(cache.read(n, count=i32(counts), start=i32(starts)), held):
+        np.testing.assert_array_equal(f64(got), x.reshape(B, n, H * 64))
+    check_clean()
+
+
+@pytest.mark.parametrize("room", [64, 700])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_many_rows_with_many_items_per_cta(cuda, bits, room):
+    """More than twenty items for each CTA, so that the entries by which its warps hear of them are used again and
+    again: items dealt out whole (room for one page) and in units."""
+    lens = [1 + 5 * b % 12 if b % 29 else 0 for b in range(640)]
+    run_case((11, 15, 5, lens, None, True, 0, 0), bits, room=room)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("case", [
+    (120, 3, 1, [1500, 700], None, True, 0, 0),       # two blocks of rows
+    (200, 3, 1, [1290, 777], [200, 90], True, 600, 70),
+    (300, 2, 2, [900], None, False, 400, 0),
+    (260, 1, 1, [2000, 0, 261], None, True, 64, 1),
+], ids=lambda c: f"r{c[0]}_w{c[6]}")
+def test_several_blocks_of_rows_over_caches_that_are_cut(cuda, case, bits):
+    run_case(case, bits)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("case", [
+    (10, 3, 1, [3000, 1500], None, True, 0, 0),       # 30 rows
+    (8, 6, 2, [2500, 40], [8, 3], True, 900, 33),     # 24 rows
+    (3, 15, 5, [2000, 2000, 1], None, False, 0, 0),   # 9 rows
+    (1, 32, 1, [4000], None, True, 0, 0),             # 32 rows
+    (4, 12, 3, [700, 90], None, True, 0, 0),          # 16 rows
+], ids=lambda c: f"r{c[0] * c[1] // c[2]}")
+def test_nine_to_32_rows_over_caches_that_are_cut(cuda, case, bits):
+    run_case(case, bits)
