@@ -100,3 +100,24 @@ def test_held_refuses_tokens_that_are_not_there(cuda):
     for first, n in ((0, 7), (5, 2), (-1, 3), (7, None), (0, -1)):
         with pytest.raises(ValueError, match="tokens"):
             text.held(0, first, n)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 10)])
+def test_what_steps_add_is_what_the_restatement_adds(cuda, bits, window, sinks):
+    """Layers whose attention weighs as much as their input, in uneven steps, against the whole sequence at once with
+    the cache's rounding; the limit is far below what a mistake costs (test_streaming_cpu.py)."""
+    from oracle import streaming_ref as O
+    from test_streaming_cpu import STEPS, strong
+    from vla_b200 import device as dev
+    from vla_b200.streaming import StreamingText
+    cfg, params, x = strong()
+    B, seq = x.shape[:2]
+    want = O.layers(x, params, cfg, bits, O.seen(seq, window, sinks))
+    text = StreamingText(cfg, params, B, seq, bits=bits, window=window, sinks=sinks)
+    got, at = [], 0
+    for n in STEPS:
+        got.append(text.step(x[:, at:at + n].reshape(B * n, -1).cuda()).view(B, n, -1))
+        at += n
+    assert O.off(torch.cat(got, 1).cpu(), want, x) < O.LIMIT[bits]
+    dev.sync_check()
