@@ -353,7 +353,9 @@ int vla_kv_read_bf16(const vla_kv_cache* c, void* k, int64_t k_row, int64_t k_ba
  * rows i >= q_len[b], are written as zeros.  Keys that are not seen have no
  * effect, whatever their memory holds.  Sequences may share queries (q_batch 0);
  * their outputs must lie apart.  scale > 0, finite also times log2(e); scores
- * count in fp32, so their magnitude has to stay below 2^30.
+ * count in fp32, so their magnitude has to stay below 2^30.  Sums are taken with
+ * probabilities of at most 2^8 and divided at the end: 2^8 times a row's keys times
+ * their largest value has to stay below 2^128.
  * max_len (0: the table's capacity) is an upper bound of lens that the split of
  * the work is made for; longer sequences stay right.  The workspace
  * (vla_kv_attention_workspace bytes, 16-byte aligned; 0: none) holds the parts'

@@ -23,7 +23,12 @@
 // would allow 88 % of the copy rate; it is 58 % busy, the rest being dependent
 // issue and the ends of the shares.  One token over 64 caches of up to 16001 keys
 // (B200, 15 / 5 heads, 4 bits): 61 us, 3.8 TB/s, 0.58 of the measured copy; 96
-// windows of 4096 keys in 8 bits with 32 / 8 heads: 87 us, 5.1 TB/s, 0.79.
+// windows of 4096 keys in 8 bits with 32 / 8 heads: 87 us, 5.1 TB/s, 0.79 (in a
+// graph; called one by one over caches of 2.5 GB in turn 91 to 96).
+// More rows take two or four 8-row tiles (64 caches of 8000 keys, 5 kv heads, 4 / 8
+// bits): 8 rows 54 / 72 us, 16 rows 78 / 90, 32 rows 124 / 132.  Four tiles in 4
+// bits want more than the 255 registers that a thread has: 192 bytes spill (172 with
+// the product taken twice; in 8 bits 0 and 12).
 // Steps that led here, on the first of these: registers instead of the ring
 // 84.6 us, ring 67.9 with one-instruction masks (89.9 with two), even shares
 // 63.9, cuts joined from records 61.2.  Slower: shifts as multiplications on the

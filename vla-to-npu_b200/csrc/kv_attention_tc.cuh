@@ -29,10 +29,14 @@
 //                loads, exponentials and packing, not any pipe, is what a unit waits
 //                for: with one thread per row (eight warps) 1024 rows over 4 x 8192 keys
 //                took 190 us.
-// What bounds it.  A unit (256 rows x 128 keys) takes about 5000 SM cycles: the
-// exponentials alone are 2048 on the MUFU (49 % busy), the tensor pipe 1000; 69 %
-// of the issue slots are used, a third of them by waiting warps.  1024 rows over 4
-// caches of up to 8192 keys (15 / 5 heads, 4 bits): 172 us, 463 TFLOP/s.  One-unit
+// What bounds it.  A unit (256 rows x 128 keys) takes about 5000 SM cycles, and no
+// pipe is full: the exponentials are 2048 of them on the MUFU (49 % busy), the tensor
+// pipe 1200; 70 % of the issue slots are used, a third of them by waiting warps.  It
+// is a row's chain: three TMEM loads that are each waited for, the maxima's swap, the
+// exponentials, the store.  1024 rows over 4 caches of up to 8192 keys (15 / 5 heads, 4
+// bits): 173 us, 461 TFLOP/s.  A block takes that time however many of its rows are
+// there: 33 rows over 64 x 8000 keys (5 heads) 265 us, 128 rows 270, 150 rows 299 (8
+// bits: 276, 284, 320).  One-unit
 // items are one chain of latencies each, about 8000 cycles (queries, scores, maximum,
 // exponentials, the last item's rows): 50 rows over each of 256 prefixes of up to 113
 // keys 54 us (66 with the rows out before the next scores and all units dealt out); 50

@@ -157,6 +157,12 @@ static int plan_attention(const vla_kv_cache* c, const vla_kv_attention_args* a,
   const long long rows = (long long)a->Lq * (a->Hq / c->kv_heads);
   VLA_CHECK_ARG(rows < (1ll << 30), "kv_attention: too many query rows");
   const int G = a->Hq / c->kv_heads;
+  // Few rows to mma.sync, by the least tile that holds them; above 32 to tcgen05, whose
+  // blocks of 256 rows take nearly the same time however few are filled.  Both sides of the
+  // border (us, 5 kv heads, 4 bits): 32 rows over 64 x 8000 keys 124 here and 250 there, 17
+  // rows over 256 x 113 keys 45 and 42 (8 bits 42 and 43); in blocks of 32, 33 rows over 256
+  // x 113 keys would take 78 and take 43 there, over 64 x 8000 keys 211 and 265, 96 rows 310
+  // and 271.
   out->nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
   const int block = out->nt > 0 ? 8 * out->nt : tc::kRows;
   const long long blocks = (rows + block - 1) / block;

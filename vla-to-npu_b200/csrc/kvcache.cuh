@@ -251,7 +251,7 @@ __device__ __forceinline__ Lane lane_of(int start, int valid, int quad, int lane
 // rows (15 / 5 heads, 4 bits), written and read back, take 26.5 us of which the bytes
 // need 15; 16 x 4001 rows in 8 bits 48 of 39 us.  Four CTAs per SM cost it 3 spilled
 // registers at most and gain a resident CTA: three 27.2 and 50.0 us, five (more
-// spills) 27.3 and 50.6.  Reading alone comes to 0.92 of the measured copy rate (32 x
+// spills) 27.3 and 50.6.  Reading alone comes to 0.91 of the measured copy rate (32 x
 // 8001 tokens, 65 us).
 template <int BITS, int QUADS>
 __global__ void __launch_bounds__(256, QUADS == 4 ? 4 : 1) append_kernel(AppendParams p) {

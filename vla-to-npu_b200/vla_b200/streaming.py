@@ -7,7 +7,10 @@ layer makes them, and its queries attend over the cache, over everything or over
 the instruction's first tokens and a window of recent ones.  The layers' weights,
 products and norms are those of ``vla_llama_self_layer_bf16`` (RMSNorm, QKV with
 RoPE, attention, output projection, RMSNorm, SwiGLU), with positions that go on
-from step to step.
+from step to step.  All streams take the same number of tokens in a step; the
+cache holds ``max_len`` tokens of each, also those that a window has left behind.
+The position is the host's, so a step is not one to capture and replay (the
+cache's own calls are).
 
     python -m vla_b200.streaming --batch 8 --steps 20 --window 1130 --sinks 48
 """
